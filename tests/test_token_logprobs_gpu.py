@@ -1,0 +1,211 @@
+"""GPU: ops.token_logprobs against the formulas in float64.
+
+Bounds: the sums of a row have at most 32 c + 16 rounded additions one after another (32 elements a thread and pass, c passes of the row, then a tree), each 2^-24
+relative, exp2 and its argument are off by 2^-23 (2 + |x - m|) relative, so log l by e = 2^-23 (32 c + 18 + max|x - m|) and log p by e + 2^-23 |x - m|. The entropy
+log l - s / l carries e from its first term and e (1 + H) from the second. A gradient adds its own rounding (eps / 2; float16 at least 2^-25)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+INF = float("inf")
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "GPU tests need a MI355X"
+    from vln_imagine_amd import ops as o
+    return o
+
+
+def _rand(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).cuda()
+
+
+def _check(ops, x, target, top, ignore=-100, seed=0, use=(True, True)):
+    V = x.shape[-1]
+    lg = x.detach().requires_grad_(True)
+    logp, ent, tl, ti = ops.token_logprobs(lg, target, top=top, ignore_index=ignore)
+    x2, t2 = x.detach().double().reshape(-1, V), target.reshape(-1)
+    dead = (x2 == -INF).all(1)
+    m = torch.where(dead, torch.zeros_like(x2[:, 0]), x2.amax(1))[:, None]
+    fin = x2 > -INF
+    z = torch.where(fin, x2 - m, torch.zeros_like(x2))
+    e = torch.where(fin, z.exp(), torch.zeros_like(z))
+    logl = torch.where(dead, torch.ones_like(m[:, 0]), e.sum(1)).log()[:, None]
+    lp = torch.where(fin, z - logl, torch.full_like(z, -INF))
+    p = torch.where(fin, (z - logl).exp(), torch.zeros_like(z))
+    plp = torch.where(fin, p * (z - logl), torch.zeros_like(z))
+    H = -plp.sum(1)
+    chunks = -(-(V + 8) // (32768 if V > 8184 else 8192 if V > 2040 else 2048))
+    far = z.abs().amax(1)
+    err = 2.0 ** -23 * (32 * chunks + 18 + far)
+    ok = (t2 >= 0) & (t2 < V) & (t2 != ignore)
+    pick = torch.where(ok, t2, torch.zeros_like(t2))[:, None]
+    want = torch.where(ok, lp.gather(1, pick)[:, 0], torch.zeros_like(H))
+    got = logp.detach().double().reshape(-1)
+    live = torch.isfinite(want)
+    assert (torch.isfinite(got) == live).all()
+    assert ((got - want).abs()[live] <= (err + 2.0 ** -23 * (far + 1))[live]).all(), ("logp", (got - want).abs()[live].max())
+    gote = ent.detach().double().reshape(-1)
+    assert ((gote - H).abs() <= err * (3 + H)).all(), ("entropy", (gote - H).abs().max())
+    assert (gote[dead] == 0).all()
+    if top:
+        order = torch.sort(x2, dim=1, descending=True, stable=True)[1][:, :top]
+        assert torch.equal(ti.reshape(-1, top), order)
+        w, g = lp.gather(1, order), tl.double().reshape(-1, top)
+        lv = torch.isfinite(w)
+        assert (torch.isfinite(g) == lv).all() and ((g - w).abs()[lv] <= (err + 2.0 ** -23 * (far + 1))[:, None].expand_as(w)[lv]).all()
+        assert not tl.requires_grad
+    else:
+        assert tl is None and ti is None
+    ga, gb = _rand(logp.shape, F32, seed + 1), _rand(logp.shape, F32, seed + 2)
+    outs = [o for o, u in ((logp, use[0]), (ent, use[1])) if u]
+    (dx,) = torch.autograd.grad(outs, [lg], [g for g, u in ((ga, use[0]), (gb, use[1])) if u])
+    a = torch.where(ok & ~dead, ga.double().reshape(-1) * use[0], torch.zeros_like(H))[:, None]
+    b = gb.double().reshape(-1)[:, None] * use[1]
+    ref = -p * a - b * (plp + p * H[:, None])
+    ref.scatter_add_(1, pick, a)
+    # (a p below the normal range, 2^-126, may come out of exp2 as 0: an absolute error of 2^-126 times the same factor)
+    slack = (2 * err[:, None] * p + 2.0 ** -126) * (a.abs() + b.abs() * (4 + H[:, None] + torch.where(fin, lp.abs(), torch.zeros_like(lp))))
+    u = torch.finfo(x.dtype).eps / 2
+    bound = u * ref.abs() + (1 + u) * (slack + 2.0 ** -22 * a.abs() * torch.zeros_like(ref).scatter_(1, pick, 1.0)) + (2.0 ** -25 if x.dtype == F16 else 1e-37)
+    assert dx.dtype == x.dtype and dx.shape == x.shape
+    d = (dx.double().reshape(-1, V) - ref).abs()
+    assert (d <= bound).all(), ("gradient", d.max(), (d / bound).max())
+    return dx
+
+
+SIZES = [1, 2, 5, 37, 64, 511, 512, 513, 1000, 2039, 2041, 2048, 4100, 8183, 8191, 8193, 30522, 32767, 40001, 70001]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("V", SIZES)
+def test_sizes(ops, dtype, V):
+    rows = 3 if V > 20000 else 7
+    x = _rand((rows, V), dtype, V, 2.0)
+    target = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(1)).cuda()
+    target[0] = -100
+    _check(ops, x, target, min(V, 5), seed=V)
+    _check(ops, x, target, 0, seed=V)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,top", [(37, 16), (16, 16), (300, 1), (1500, 8), (6000, 16), (30522, 8), (66000, 3)])
+def test_ties_masks_and_empty_rows(ops, dtype, V, top):
+    """Few distinct values (ties everywhere: lowest index first), impossible entries at -inf, a row of them only, one with fewer than `top` possible ones."""
+    rows = 6
+    x = torch.randint(-2, 3, (rows, V), generator=torch.Generator().manual_seed(V)).to(dtype).cuda()
+    x[1, torch.rand(V, generator=torch.Generator().manual_seed(2)).cuda() < 0.6] = -INF
+    x[2] = -INF
+    x[3] = -INF
+    x[3, V // 2] = 1.5
+    x[4] = 0.0
+    x[4, V // 3] = -0.0
+    target = torch.tensor([0, V - 1, 0, V // 2, V // 3, -100]).cuda()
+    target[1] = int((x[1] > -INF).nonzero()[0])
+    dx = _check(ops, x, target, top)
+    assert (dx[2] == 0).all() and torch.isfinite(dx.float()).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_strides_and_starts(ops, dtype):
+    """Rows with a gap behind them, rows that start anywhere, a transposed matrix, a batch of sequences, one row without an axis."""
+    V, rows = 1003, 9
+    t = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(1)).cuda()
+    wide = _rand((rows, V + 61), dtype, 1)
+    for s in (0, 1, 3, 61):
+        _check(ops, wide[:, s:s + V], t, 4)
+    keep = wide.clone()
+    ops.token_logprobs(wide[:, 3:3 + V].requires_grad_(True), t, top=2)[0].sum().backward()
+    assert torch.equal(wide, keep)
+    _check(ops, _rand((V, rows), dtype, 2).t(), t, 4)
+    flat = _rand((rows * V + 5,), dtype, 3)
+    for s in (1, 2, 5):
+        _check(ops, flat[s:s + rows * V].view(rows, V), t, 4)
+    _check(ops, _rand((3, 3, V), dtype, 4), t.view(3, 3), 2)
+    _check(ops, _rand((2, 3, V + 5), dtype, 4)[..., :V], t[:6].view(2, 3), 2)
+    _check(ops, _rand((V,), dtype, 5), t[0], 3)
+
+
+def test_large_values_and_offsets(ops):
+    x = _rand((4, 3001), F32, 1, 30.0)
+    x[1] += 1e6
+    x[2] -= 1e6
+    t = torch.tensor([5, 6, 7, 8]).cuda()
+    _check(ops, x, t, 3)
+
+
+@pytest.mark.parametrize("use", [(True, False), (False, True)])
+def test_one_gradient_only(ops, use):
+    _check(ops, _rand((5, 700), BF16, 1), torch.arange(5).cuda(), 0, use=use)
+
+
+def test_ignored_and_out_of_range_targets(ops):
+    x = _rand((6, 50), F32, 1)
+    ops.watch_index_errors()
+    ops.index_errors(raise_=False)
+    _check(ops, x, torch.tensor([0, 0, 3, 49, 0, 7]).cuda(), 2, ignore=0)          # a padding id that is a valid column
+    assert ops.index_errors(raise_=False) == 0
+    _check(ops, x, torch.tensor([50, -1, 3, 49, -100, 1 << 40]).cuda(), 2)
+    with pytest.raises(IndexError):
+        ops.index_errors()
+    assert ops.index_errors() == 0
+
+
+def test_no_rows(ops):
+    x = torch.empty((0, 40), device="cuda", requires_grad=True)
+    logp, ent, tl, ti = ops.token_logprobs(x, torch.empty((0,), dtype=torch.int64, device="cuda"), top=2)
+    assert logp.shape == (0,) and tl.shape == (0, 2)
+    (logp.sum() + ent.sum()).backward()
+    assert x.grad.shape == (0, 40)
+
+
+def test_expanded_gradient_and_equal_bits(ops):
+    x = _rand((64, 5000), BF16, 3).requires_grad_(True)
+    t = torch.arange(64).cuda()
+    a = torch.autograd.grad(ops.token_logprobs(x, t)[0].sum(), x)[0]
+    b = torch.autograd.grad(ops.token_logprobs(x, t)[0], x, torch.ones(64, device="cuda"))[0]
+    assert torch.equal(a, b)
+
+
+def test_captured_and_replayed(ops):
+    x, t = _rand((40, 9000), BF16, 1), torch.arange(40).cuda()
+    g1, g2 = _rand((40,), F32, 2), _rand((40,), F32, 3)
+
+    def step():
+        lg = x.detach().requires_grad_(True)
+        lp, ent, tl, ti = ops.token_logprobs(lg, t, top=4)
+        return [lp.detach(), ent.detach(), tl, ti, torch.autograd.grad([lp, ent], [lg], [g1, g2])[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = step()
+    for r in range(3):
+        x.copy_(_rand(x.shape, BF16, 10 + r))
+        t.copy_(torch.randint(0, 9000, (40,), generator=torch.Generator().manual_seed(r)))
+        g.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(res, want)), r
+
+
+def test_gradient_against_differences(ops):
+    """float32, V = 50: a step of 2^-5 along a unit direction leaves a cubic error below 1e-3 and a rounding error of 2^-22 / 2^-4."""
+    x, t = _rand((3, 50), F32, 1), torch.tensor([4, 5, 6]).cuda()
+    lg = x.clone().requires_grad_(True)
+    lp, ent, _, _ = ops.token_logprobs(lg, t)
+    (lp.sum() + 0.7 * ent.sum()).backward()
+    d = _rand(x.shape, F32, 9)
+    d /= d.norm()
+    h = 2.0 ** -5
+    val = []
+    for s in (h, -h):
+        lp, ent, _, _ = ops.token_logprobs(x + s * d, t)
+        val.append(lp.double().sum() + 0.7 * ent.double().sum())
+    assert abs(((val[0] - val[1]) / (2 * h)).item() - (lg.grad.double() * d.double()).sum().item()) < 2e-3

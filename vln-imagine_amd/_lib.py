@@ -89,6 +89,9 @@ SIGNATURES = {
     "vlni_scale_cast": [I, I, P, P, L, F, P],
     "vlni_embed_combine_fwd": [I, P, L, P, P, P, L, I, P, P, P, P, P, L, P, P, P, I, P, P, I, P, P, F, P, P, P, L, P, P, P, P, P, P, F, U, I, I, P],
     "vlni_ln_rowdot_fwd": [I, P, L, P, P, F, P, P, P, P, P, P, P, F, U, I, I, P],
+    "vlni_long_attn_sizes": [P, P], "vlni_long_attn_fwd": [P, P], "vlni_long_attn_bwd": [P, P],
+    "vlni_token_logprobs_fwd": [I, P, L, P, L, P, P, P, P, P, I, I, I, P],
+    "vlni_token_logprobs_bwd": [I, P, P, P, L, P, L, P, P, L, I, I, P],
     "vlni_self_att_block_fwd": [P, P], "vlni_self_att_block_bwd": [P, P], "vlni_ffn_block_fwd": [P, P], "vlni_ffn_block_bwd": [P, P],
 }
 

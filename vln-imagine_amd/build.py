@@ -9,14 +9,15 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libvlni.so")
-SOURCES = ["api.hip", "gemm.hip", "layernorm.hip", "elementwise.hip", "attention.hip", "graphmap.hip", "blocks.hip"]
+SOURCES = ["api.hip", "gemm.hip", "layernorm.hip", "elementwise.hip", "attention.hip", "graphmap.hip", "blocks.hip",
+           "long_attention.hip", "long_attention_f16.hip", "long_attention_f32.hip", "logprobs.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
          # no packed float32 instructions (v_pk_fma_f32 ...): some of their forms have given wrong results on gfx950, without an error. They
          # round like the scalar ones, so results are unchanged. The host pass does not know the feature and says so: harmless
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-source flags. attention.hip: MFMA results in VGPRs - with the accumulators in AGPRs every softmax operation on a score tile is an
 # accvgpr read + write around it (448 of the forward kernel's 1872 VALU instructions, 144 registers instead of 113: -16 % per launch)
-EXTRA = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+EXTRA = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for s in ("attention.hip", "long_attention.hip", "long_attention_f16.hip", "long_attention_f32.hip")}
 if os.environ.get("VLNI_DIAG") == "1":       # stamped / timing-only kernel builds + vlni_debug_pk_stamps (tools/gemm_stamps.py); never the default
     FLAGS.append("-DVLNI_DIAG")
 
@@ -36,12 +37,14 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    hdrs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".inc"))]     # *_impl.inc: kernel bodies included per 16-bit type
+    hdrs = [f for f in os.listdir(CSRC) if f.endswith((".h", ".inc"))]     # *_impl.inc: kernel bodies included per 16-bit type
     jobs = []
     for s in SOURCES:
         src = os.path.join(CSRC, s)
         obj = os.path.join(objdir, s.replace(".hip", ".o"))
-        if force or _stale(obj, [src] + hdrs + [os.path.abspath(__file__)]):
+        # long_attention*.{h,inc} are included by the long_attention*.hip sources only
+        deps = [os.path.join(CSRC, f) for f in hdrs if not f.startswith("long_attention") or s.startswith("long_attention")]
+        if force or _stale(obj, [src] + deps + [os.path.abspath(__file__)]):
             jobs.append((src, obj))
 
     def cc(job):

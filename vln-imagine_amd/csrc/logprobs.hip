@@ -1,0 +1,273 @@
+// Log probabilities of given tokens with the entropy of their rows and the most likely alternatives, and their gradient (ops.token_logprobs).
+//
+//   m = max x, l = sum exp(x - m), s = sum exp(x - m)(x - m);  logp_t = x_t - m - log l;  H = log l - s / l     (differences from m: no cancellation
+//   dx_v = g ([v = t] - p_v) - h p_v (log p_v + H)                                                              of large offsets)
+//
+// Bound by memory: forward reads the logits once - a thread keeps its own running (m, l, s), merged over the row at the end -, backward reads
+// them once and writes the gradient; nothing else of the logits' size is made. Rows start at any element (30522 16-bit columns are no multiple
+// of 16 bytes): vectors are laid on the row's 16-byte boundaries, and the partial ones at its ends are read and written element by element.
+//
+// Alternatives: a row (or 32 k of it at a time) sits in registers, so the best is taken out `top` times; a 64-bit key (order-preserving bits of
+// x, then the complement of the index) makes "largest value, lowest index" one comparison. Only the wave that lost its best looks again.
+#include "../../include/vlni.h"
+#include "common.h"
+
+namespace {
+
+constexpr int LP_MAXTOP = 16;
+constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
+typedef unsigned long long u64;
+
+struct LpP {
+  const void* x; long ld;
+  const long* target; long ignore;
+  float *logp, *ent, *stat;            // stat [rows][3]: m, log l, H
+  float* top_logp; long* top_idx;
+  int rows, V, top;
+  int* bad;                            // counter of targets outside [0, V), or null
+  // backward
+  const float *g, *h;                  // gradients of logp and of the entropy (either null)
+  void* dx; long lddx;
+};
+
+__device__ __forceinline__ unsigned lp_order(float x) {                      // monotone: -inf < ... < +inf (-0 = 0)
+  const unsigned u = __float_as_uint(x + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float lp_value(u64 key) {
+  const unsigned o = (unsigned)(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ u64 lp_wave_max(u64 k) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const u64 other = ((u64)(unsigned)__shfl_xor((int)(k >> 32), o, 64) << 32) | (unsigned)__shfl_xor((int)k, o, 64);
+    k = other > k ? other : k;
+  }
+  return k;
+}
+// (m, l, s) of two parts of a row; a part without elements has m = -inf, l = s = 0
+__device__ __forceinline__ void lp_merge(float& m, float& l, float& s, float m2, float l2, float s2) {
+  const float mn = fmaxf(m, m2), mu = mn == -INFINITY ? 0.f : mn;
+  const float d1 = fmaxf(m - mu, -1e30f), d2 = fmaxf(m2 - mu, -1e30f);       // an empty part's weight is 0, not 0 * inf
+  const float w1 = __builtin_amdgcn_exp2f(d1 * LP_LOG2E), w2 = __builtin_amdgcn_exp2f(d2 * LP_LOG2E);
+  s = (s + l * d1) * w1 + (s2 + l2 * d2) * w2;
+  l = l * w1 + l2 * w2;
+  m = mn;
+}
+
+// 16 / sizeof(T) elements of a row from element e on; those outside [0, V) are -inf. Only whole vectors inside the row are read as vectors.
+template <typename T, int VEC> __device__ __forceinline__ void lp_load(float (&x)[VEC], const T* row, long e, int V) {
+  if constexpr (VEC == 1) {
+    x[0] = e < V ? (float)row[e] : -INFINITY;
+  } else {
+    if (e >= 0 && e + VEC <= V) {
+      typedef T vec __attribute__((ext_vector_type(VEC)));
+      const vec v = *(const vec*)(row + e);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[j] = (float)v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[j] = e + j >= 0 && e + j < V ? (float)row[e + j] : -INFINITY;
+    }
+  }
+}
+template <typename T> __device__ __forceinline__ int lp_head(const T* row) {      // elements between the 16-byte boundary below the row and the row
+  return (int)(((uintptr_t)row & 15) / sizeof(T));
+}
+
+// TPB threads per row (64: four rows a block), N vectors of VEC elements a thread and pass
+template <typename T, int TPB, int VEC, int N, bool TOP>
+__global__ __launch_bounds__(TPB < 256 ? 256 : TPB) void lp_fwd_kernel(LpP p) {
+  constexpr int NW = TPB / 64;                       // waves of a row
+  __shared__ u64 wbest[16];
+  __shared__ float red[3][16];
+  const int tid = threadIdx.x % TPB, lane = threadIdx.x & 63, wave = NW == 1 ? 0 : tid >> 6;
+  const long row_i = NW == 1 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (NW == 1 && row_i >= p.rows) return;
+  const T* row = (const T*)p.x + row_i * p.ld;
+  const long e0 = VEC == 1 ? 0 : -lp_head(row);
+  float m = -INFINITY, l = 0.f, s = 0.f;
+  u64 list = 0;                                      // lane q of every wave: the q-th best so far
+  for (long c0 = e0; c0 < p.V; c0 += (long)TPB * N * VEC) {
+    float x[N][VEC];
+#pragma unroll
+    for (int n = 0; n < N; ++n) lp_load<T, VEC>(x[n], row, c0 + ((long)n * TPB + tid) * VEC, p.V);
+    float mt = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) mt = fmaxf(mt, x[n][j]);
+    const float mu = mt == -INFINITY ? 0.f : mt;
+    float lt = 0.f, st = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float d = x[n][j] - mu, e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+        lt += e;
+        st += e * fmaxf(d, -1e30f);
+      }
+    lp_merge(m, l, s, mt, lt, st);
+    if constexpr (TOP) {
+      unsigned taken = 0;
+      auto own = [&]() {
+        u64 k = 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const long e = c0 + ((long)n * TPB + tid) * VEC + j;
+            const u64 key = ((u64)lp_order(x[n][j]) << 32) | (0xFFFFFFFFu - (unsigned)e);
+            if (e >= 0 && e < p.V && !(taken >> (n * VEC + j) & 1) && key > k) k = key;
+          }
+        return k;
+      };
+      u64 mine = own(), wmax = lp_wave_max(mine);
+      if (NW > 1) {
+        __syncthreads();
+        if (lane == 0) wbest[wave] = wmax;
+        __syncthreads();
+      }
+      while (true) {
+        const u64 k = NW == 1 ? wmax : lp_wave_max(lane < NW ? wbest[lane] : 0);
+        const u64 last = ((u64)(unsigned)__shfl((int)(list >> 32), p.top - 1, 64) << 32) | (unsigned)__shfl((int)list, p.top - 1, 64);
+        if (k <= last) break;                          // the row is used up (0), or nothing beats the last alternative
+        const u64 prev = ((u64)(unsigned)__shfl_up((int)(list >> 32), 1, 64) << 32) | (unsigned)__shfl_up((int)list, 1, 64);
+        if (list < k) list = lane == 0 || prev > k ? k : prev;
+        // the owner drops it
+        if (NW > 1) __syncthreads();
+        if (wmax == k) {                             // (keys are unique: one wave)
+          if (mine == k) {
+            const long e = (long)(0xFFFFFFFFu - (unsigned)k) - c0;
+            const int n = (int)(e / VEC / TPB), j = (int)(e % VEC);
+            taken |= 1u << (n * VEC + j);
+            mine = own();
+          }
+          wmax = lp_wave_max(mine);
+          if (NW > 1 && lane == 0) wbest[wave] = wmax;
+        }
+        if (NW > 1) __syncthreads();
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64), s2 = __shfl_xor(s, o, 64);
+    lp_merge(m, l, s, m2, l2, s2);
+  }
+  if (NW > 1) {
+    if (lane == 0) { red[0][wave] = m; red[1][wave] = l; red[2][wave] = s; }
+    __syncthreads();
+    m = red[0][0]; l = red[1][0]; s = red[2][0];
+    for (int w = 1; w < NW; ++w) lp_merge(m, l, s, red[0][w], red[1][w], red[2][w]);
+  }
+  const bool dead = m == -INFINITY && l == 0.f;                                  // nothing but -inf
+  const float logl = dead ? 0.f : __builtin_amdgcn_logf(l) * LP_LN2, H = dead ? 0.f : logl - s / l;
+  if (tid == 0) {
+    const long t = p.target[row_i];
+    float lp = 0.f;
+    if (t >= 0 && t < p.V) lp = dead ? -INFINITY : ((float)row[t] - m) - logl;
+    else if (t != p.ignore && p.bad) atomicAdd(p.bad, 1);
+    p.logp[row_i] = t == p.ignore ? 0.f : lp;
+    p.ent[row_i] = H;
+    p.stat[3 * row_i] = m;
+    p.stat[3 * row_i + 1] = logl;
+    p.stat[3 * row_i + 2] = H;
+  }
+  if (TOP && wave == 0 && lane < p.top) {
+    p.top_idx[row_i * p.top + lane] = (long)(0xFFFFFFFFu - (unsigned)list);
+    p.top_logp[row_i * p.top + lane] = dead ? -INFINITY : (lp_value(list) - m) - logl;
+  }
+}
+
+// grid = (rows / rows a block, parts of a row); TPB threads per row and part
+template <typename T, int TPB, int VEC, int N>
+__global__ __launch_bounds__(256) void lp_bwd_kernel(LpP p) {
+  const int tid = threadIdx.x % TPB;
+  const long row_i = (long)blockIdx.x * (256 / TPB) + threadIdx.x / TPB;
+  if (row_i >= p.rows) return;
+  const T* row = (const T*)p.x + row_i * p.ld;
+  T* out = (T*)p.dx + row_i * p.lddx;
+  const long e0 = VEC == 1 ? 0 : -lp_head(row);
+  const bool same = VEC > 1 && lp_head(row) == lp_head(out);
+  const float m = p.stat[3 * row_i], logl = p.stat[3 * row_i + 1], H = p.stat[3 * row_i + 2];
+  const long t = p.target[row_i];
+  const bool dead = m == -INFINITY && logl == 0.f, scored = t >= 0 && t < p.V && t != p.ignore;
+  const float g = p.g && scored && !dead ? p.g[row_i] : 0.f, h = p.h ? p.h[row_i] : 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const long e = e0 + (long)blockIdx.y * TPB * N * VEC + ((long)n * TPB + tid) * VEC;
+    if (e >= p.V) break;
+    float x[VEC];
+    lp_load<T, VEC>(x, row, e, p.V);
+    T v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float lp = (x[j] - m) - logl, pr = __builtin_amdgcn_exp2f(lp * LP_LOG2E);
+      float d = -pr * (g + h * (fmaxf(lp, -1e30f) + H));
+      if (e + j == t) d += g;
+      v[j] = (T)(dead ? 0.f : d);
+    }
+    if constexpr (VEC > 1) {
+      if (same && e >= 0 && e + VEC <= p.V) {
+        typedef T vec __attribute__((ext_vector_type(VEC)));
+        vec w;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w[j] = v[j];
+        *(vec*)(out + e) = w;
+        continue;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (e + j >= 0 && e + j < p.V) out[e + j] = v[j];
+  }
+}
+
+template <typename T, bool TOP> int lp_fwd_launch(const LpP& p, hipStream_t st) {
+  constexpr int CE = 16 / (int)sizeof(T);
+  // a wave per row while a row fits its registers; short rows element by element (their vectors would be mostly partial)
+  if (p.V <= 512) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, 1, 8, TOP>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
+  else if (p.V <= 2048 - CE) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, CE, 32 / CE, TOP>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
+  else if (p.V <= 8192 - CE) hipLaunchKernelGGL((lp_fwd_kernel<T, 256, CE, 32 / CE, TOP>), dim3(p.rows), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((lp_fwd_kernel<T, 1024, CE, 32 / CE, TOP>), dim3(p.rows), dim3(1024), 0, st, p);
+  VLNI_LAUNCH_CHECK();
+  return VLNI_OK;
+}
+template <typename T> int lp_bwd_launch(const LpP& p, hipStream_t st) {
+  constexpr int CE = 16 / (int)sizeof(T);
+  if (p.V <= 512) hipLaunchKernelGGL((lp_bwd_kernel<T, 64, 1, 8>), dim3(cdiv(p.rows, 4), 1), dim3(256), 0, st, p);
+  else if (p.V <= 2048 - CE) hipLaunchKernelGGL((lp_bwd_kernel<T, 64, CE, 32 / CE>), dim3(cdiv(p.rows, 4), 1), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((lp_bwd_kernel<T, 256, CE, 32 / CE>), dim3(p.rows, cdiv((long)p.V + CE, 8192)), dim3(256), 0, st, p);
+  VLNI_LAUNCH_CHECK();
+  return VLNI_OK;
+}
+}  // namespace
+
+extern "C" int vlni_token_logprobs_fwd(int dtype, const void* logits, long ld, const long* target, long ignore_index, float* logp, float* entropy,
+                                       float* stat, float* top_logp, long* top_index, int top, int rows, int V, void* stream) {
+  VLNI_CHECK(dtype >= VLNI_F32 && dtype <= VLNI_F16, VLNI_EINVAL, "token_logprobs: dtype %d", dtype);
+  VLNI_CHECK(rows > 0 && V > 0 && V < (1 << 30) && ld >= V, VLNI_EINVAL, "token_logprobs: rows=%d V=%d ld=%ld", rows, V, ld);
+  VLNI_CHECK(top >= 0 && top <= LP_MAXTOP && top <= V, VLNI_EUNSUP, "token_logprobs: top=%d of %d (at most %d)", top, V, LP_MAXTOP);
+  VLNI_CHECK(logits && target && logp && entropy && stat && (!top || (top_logp && top_index)), VLNI_EINVAL, "token_logprobs: null pointer");
+  LpP p{};
+  p.x = logits; p.ld = ld; p.target = target; p.ignore = ignore_index; p.logp = logp; p.ent = entropy; p.stat = stat; p.top_logp = top_logp;
+  p.top_idx = top_index; p.rows = rows; p.V = V; p.top = top; p.bad = vlni_index_error_counter();
+  const hipStream_t st = (hipStream_t)stream;
+#define LP_GO(T) (top ? lp_fwd_launch<T, true>(p, st) : lp_fwd_launch<T, false>(p, st))
+  return dtype == VLNI_F32 ? LP_GO(float) : dtype == VLNI_BF16 ? LP_GO(__bf16) : LP_GO(_Float16);
+#undef LP_GO
+}
+
+extern "C" int vlni_token_logprobs_bwd(int dtype, const float* dlogp, const float* dentropy, const void* logits, long ld, const long* target,
+                                       long ignore_index, const float* stat, void* dlogits, long lddl, int rows, int V, void* stream) {
+  VLNI_CHECK(dtype >= VLNI_F32 && dtype <= VLNI_F16, VLNI_EINVAL, "token_logprobs: dtype %d", dtype);
+  VLNI_CHECK(rows > 0 && V > 0 && V < (1 << 30) && ld >= V && lddl >= V, VLNI_EINVAL, "token_logprobs: rows=%d V=%d ld=%ld lddl=%ld", rows, V, ld, lddl);
+  VLNI_CHECK(logits && target && stat && dlogits, VLNI_EINVAL, "token_logprobs: null pointer");
+  LpP p{};
+  p.x = logits; p.ld = ld; p.target = target; p.ignore = ignore_index; p.stat = (float*)stat; p.rows = rows; p.V = V; p.g = dlogp; p.h = dentropy;
+  p.dx = dlogits; p.lddx = lddl;
+  const hipStream_t st = (hipStream_t)stream;
+  return dtype == VLNI_F32 ? lp_bwd_launch<float>(p, st) : dtype == VLNI_BF16 ? lp_bwd_launch<__bf16>(p, st) : lp_bwd_launch<_Float16>(p, st);
+}

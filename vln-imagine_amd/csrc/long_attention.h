@@ -1,0 +1,31 @@
+// Shared by long_attention.hip (entry points, bfloat16, float16) and long_attention_f32.hip.
+#pragma once
+#include "common.h"
+
+constexpr float LA_LOG2E = 1.4426950408889634f;
+constexpr float LA_LOWEST = -1e30f;          // finite masks below this count as this
+constexpr float LA_ABSORB = -1e20f;          // a running maximum below this came from such a mask
+constexpr int LA_PAD = 96;                   // a 32 x 64 piece that touches distance R reaches at most 94 beyond it
+constexpr int LA_MAXB = 64;                  // buckets per side
+
+struct LaP {
+  const void *q, *k, *v, *dout;
+  long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, d_b, d_s, d_h;      // strides in elements
+  void* out;                   // [B, Sq, nh, D]
+  float* lse; float* rl;       // [B, nh, Sq] each: see the masks' comment above
+  float* delta;                // [B, nh, Sq]
+  const float* kml;            // [B, SkP] mask in units of log2, -inf behind Sk; null without a mask
+  const int* kind;             // [B, SkP / 64]: 0 no mask in these 64 keys, 1 some, 2 nothing but -inf
+  const float* bvec;           // [nh, BL] bias by distance in units of log2, saturated LA_PAD beyond +-R; null without a bias
+  float* part; float* part_ml; // split launches: float32 partial results; running (maximum, sum)
+  void *dq, *dk, *dv;
+  float* dbpart;               // [nh][B * row blocks * splits][BL] sums of dS by distance, or null
+  int B, Sq, Sk, SkP, nh, nkv, D, causal, PG, R, BL, nblk, nsplit;
+  float c1, scale;             // c1 = scale log2(e)
+};
+
+
+// what: 0 forward, 1 dQ + delta + dS by distance, 2 dK + dV; each with the join of its splits
+int la_run_bf16(const LaP& p, int what, hipStream_t st);
+int la_run_f16(const LaP& p, int what, hipStream_t st);
+int la_run_f32(const LaP& p, int what, hipStream_t st);

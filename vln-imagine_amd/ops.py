@@ -3524,3 +3524,231 @@ def segment_mean(x2, seg_off, rowidx):
 
 def cosine(x, y):
     return _Cosine.apply(x, y)
+
+
+# =====================================================================================
+#  attention over long sequences, token log probabilities
+# =====================================================================================
+class _LongAttnArgs(ctypes.Structure):       # VlniLongAttnArgs (include/vlni.h)
+    _fields_ = [(n, ctypes.c_int) for n in ("dtype", "B", "Sq", "Sk", "nh", "nkv", "D", "causal")] + \
+               [("scale", ctypes.c_float), ("rel_n", ctypes.c_int), ("rel_sides", ctypes.c_int), ("rel_first", ctypes.c_void_p)] + \
+               [(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout")] + \
+               [(n, ctypes.c_long * 3) for n in ("q_stride", "k_stride", "v_stride", "do_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("kmask", "rel_table", "out", "stat")] + \
+               [("prep", ctypes.c_void_p), ("prep_floats", ctypes.c_long), ("work", ctypes.c_void_p), ("work_floats", ctypes.c_long)] + \
+               [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "dtable")]
+
+
+_REL_FIRST = {}
+
+
+def rel_bucket_starts(n, rel_max):
+    """Smallest distance of each of the n buckets of one side: distances below n // 2 have one bucket each, bucket n // 2 + b begins at the smallest d
+    with d >= (n // 2) (rel_max / (n // 2))^(b / (n - n // 2)) - found in whole numbers, so that no rounding moves a border. ctypes int array."""
+    a = _REL_FIRST.get((n, rel_max))
+    if a is None:
+        e = n // 2
+        first = list(range(e + 1))
+        for b in range(1, n - e):
+            d = first[-1]
+            while d ** (n - e) * e ** b < rel_max ** b * e ** (n - e):
+                d += 1
+            first.append(d)
+        a = _REL_FIRST[(n, rel_max)] = (ctypes.c_int * n)(*first)
+    return a
+
+
+def _la_view(t):
+    """t itself where the kernels can read it (the last axis contiguous, everything else on 16-byte steps), else a dense copy."""
+    step = 16 // t.element_size()
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] == 1 or (t.stride(i) % step == 0 and t.stride(i) >= 0) for i in range(3))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _la_strides(t):
+    return (ctypes.c_long * 3)(*[t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)])
+
+
+def _la_call(fn, a, device):
+    with torch.cuda.device(device):
+        _lib.call(fn, ctypes.addressof(a), _st())
+
+
+class _LongAttention(torch.autograd.Function):
+    """softmax(scale q k^T + kmask + bias by distance) v without the score matrix (vlni_long_attn_*). Saves q, k, v, out and two floats per row; the
+    backward pass recomputes the probabilities. Inside an EpisodeTape it computes in every pass, the ghost pass included (on the filled buffers)."""
+
+    @staticmethod
+    def _args(q, k, v, kmask, table, cfg):
+        causal, scale, sides, first = cfg
+        a = _LongAttnArgs()
+        a.dtype, a.B, a.Sq, a.nh, a.D = _dt(q), *q.shape
+        a.Sk, a.nkv, a.causal, a.scale = k.shape[1], k.shape[2], int(causal), scale
+        a.q, a.k, a.v, a.kmask, a.rel_table = q.data_ptr(), k.data_ptr(), v.data_ptr(), _p(kmask), _p(table)
+        a.q_stride, a.k_stride, a.v_stride = _la_strides(q), _la_strides(k), _la_strides(v)
+        if table is not None:
+            a.rel_n, a.rel_sides, a.rel_first = len(first), sides, ctypes.addressof(first)
+        sizes = (ctypes.c_long * 3)()
+        _lib.call("vlni_long_attn_sizes", ctypes.addressof(a), ctypes.addressof(sizes))
+        return a, sizes
+
+    @staticmethod
+    def forward(ctx, q, k, v, kmask, table, cfg):
+        ctx.cfg, ctx.shapes = cfg, (q.shape, k.shape)
+        ctx.empty = q.numel() == 0 or k.numel() == 0
+        if ctx.empty:
+            ctx.tshape = None if table is None else table.shape
+            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        q, k, v = _la_view(q), _la_view(k), _la_view(v)
+        kmask = None if kmask is None else kmask.contiguous()
+        table = None if table is None else table.contiguous()
+        a, sizes = _LongAttention._args(q, k, v, kmask, table, cfg)
+        B, Sq, nh, D = q.shape
+        out = torch.empty((B, Sq, nh, D), dtype=q.dtype, device=q.device)
+        stat = torch.empty((2, B, nh, Sq), dtype=torch.float32, device=q.device)
+        prep = torch.empty((sizes[0],), dtype=torch.float32, device=q.device) if sizes[0] else None
+        work = torch.empty((sizes[1],), dtype=torch.float32, device=q.device) if sizes[1] else None
+        a.out, a.stat, a.prep, a.prep_floats, a.work, a.work_floats = out.data_ptr(), stat.data_ptr(), _p(prep), sizes[0], _p(work), sizes[1]
+        _la_call("vlni_long_attn_fwd", a, q.device)
+        ctx.save_for_backward(q, k, v, kmask, table, out, stat, prep)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        ng = ctx.needs_input_grad
+        qs, ks = ctx.shapes
+        if ctx.empty:
+            z = [torch.zeros(s, dtype=dout.dtype, device=dout.device) if n else None for s, n in zip((qs, ks, ks), ng)]
+            return (*z, None, torch.zeros(ctx.tshape, dtype=torch.float32, device=dout.device) if ng[4] else None, None)
+        q, k, v, kmask, table, out, stat, prep = ctx.saved_tensors
+        dout = _la_view(dout)
+        a, sizes = _LongAttention._args(q, k, v, kmask, table, ctx.cfg)
+        dq = torch.empty(qs, dtype=q.dtype, device=q.device)
+        dk, dv = (torch.empty(ks, dtype=q.dtype, device=q.device) for _ in range(2))
+        dtable = torch.empty_like(table) if ng[4] else None
+        work = torch.empty((sizes[2],), dtype=torch.float32, device=q.device)
+        a.dout, a.do_stride = dout.data_ptr(), _la_strides(dout)
+        a.out, a.stat, a.prep, a.prep_floats, a.work, a.work_floats = out.data_ptr(), stat.data_ptr(), _p(prep), sizes[0], work.data_ptr(), sizes[2]
+        a.dq, a.dk, a.dv, a.dtable = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(dtable)
+        _la_call("vlni_long_attn_bwd", a, q.device)
+        return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, None, dtable, None
+
+
+def _same_device(t0, name0, **others):
+    _chk(t0, name0)
+    for n, t in others.items():
+        if t is not None and t.device != t0.device:
+            raise RuntimeError(f"vlni: {n} is on {t.device}, {name0} on {t0.device}")
+
+
+def long_attention(q, k, v, kmask=None, causal=False, scale=None, rel_table=None, rel_max=128, rel_bidirectional=True):
+    """Attention over sequences of any length: softmax(scale q k^T + kmask + bias) v, forward and backward without the score matrix.
+
+    q [B, Sq, nh, D], k and v [B, Sk, nkv, D] (float32, bfloat16 or float16; D a multiple of 8 up to 128; any strides - views of a packed projection
+    are read in place where they lie on 16-byte steps). nh may be a multiple of nkv: query head h reads key head h * nkv // nh. Returns [B, Sq, nh, D].
+    kmask: additive float32 [B, Sk] as `additive_mask` makes it. -inf excludes a key altogether (its k and v may hold anything), finite values are
+        added; those below -1e30 count as -1e30. A row without any key gives zeros and sends no gradient back.
+    causal: position i sees the keys j <= i + Sk - Sq (the sequences end together: one new token against a cache is Sq = 1).
+    rel_table: float32 [buckets, nh], a learned bias by the distance j - (i + Sk - Sq), looked up in the kernels and trained through them. Of the n
+        buckets of a side the first n // 2 hold one distance each, the others are spread over log(distance) up to rel_max (<= 1024), the last holds all
+        beyond (rel_bucket_starts). rel_bidirectional: the upper half of the table is for keys behind the query; otherwise those count as distance 0.
+    scale: 1 / sqrt(D) by default. Sums are float32 and in a fixed order: equal calls on one device give equal bits. No dropout, no second derivative."""
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"long_attention: {n} has shape {tuple(t.shape)}, expected [batch, positions, heads, head size]")
+    _dt(q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"long_attention: q, k, v are {q.dtype}, {k.dtype}, {v.dtype}")
+    (B, Sq, nh, D), (_, Sk, nkv, _) = q.shape, k.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"long_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if nh < 1 or nkv < 1 or nh % nkv or nh > 1024:
+        raise ValueError(f"long_attention: {nh} heads do not share {nkv} key heads evenly (at most 1024 heads)")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"long_attention: head size {D} is not a multiple of 8 up to 128")
+    if kmask is not None:
+        if kmask.dtype != torch.float32 or tuple(kmask.shape) != (B, Sk):
+            raise ValueError(f"long_attention: kmask is {kmask.dtype} {tuple(kmask.shape)}, expected additive float32 {(B, Sk)}")
+        if kmask.requires_grad:
+            raise ValueError("long_attention: kmask takes no gradient")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e6:
+        raise ValueError(f"long_attention: scale {scale}")
+    sides, first = 0, None
+    if rel_table is not None:
+        if rel_table.dtype != torch.float32 or rel_table.dim() != 2 or rel_table.shape[1] != nh:
+            raise ValueError(f"long_attention: rel_table is {rel_table.dtype} {tuple(rel_table.shape)}, expected float32 [buckets, {nh}]")
+        sides = 2 if rel_bidirectional else 1
+        n = rel_table.shape[0] // sides
+        if rel_table.shape[0] % sides or not 2 <= n <= 64:
+            raise ValueError(f"long_attention: {rel_table.shape[0]} buckets on {sides} side(s): 2 to 64 a side")
+        if int(rel_max) != rel_max or not n // 2 < rel_max <= 1024:
+            raise ValueError(f"long_attention: rel_max {rel_max} with {n} buckets a side: a whole number above {n // 2}, at most 1024")
+        first = rel_bucket_starts(n, int(rel_max))
+    _same_device(q, "q", k=k, v=v, kmask=kmask, rel_table=rel_table)
+    return _LongAttention.apply(q, k, v, kmask, rel_table, (bool(causal), scale, sides, first))
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    """(log p[target], entropy, top log probabilities, their indices) of every row (vlni_token_logprobs_*); saves the logits and three floats a row."""
+
+    @staticmethod
+    def forward(ctx, logits, target, top, ignore_index):
+        shp, V = logits.shape[:-1], logits.shape[-1]
+        x = _rows(logits)
+        rows, dev = x.shape[0], x.device
+        t = target.reshape(-1).contiguous()
+        logp, ent = (torch.empty((rows,), dtype=torch.float32, device=dev) for _ in range(2))
+        stat = torch.empty((rows, 3), dtype=torch.float32, device=dev)
+        tl = torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None
+        ti = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
+        if rows:
+            with torch.cuda.device(dev):
+                _lib.call("vlni_token_logprobs_fwd", _dt(x), x.data_ptr(), x.stride(0), t.data_ptr(), ignore_index, logp.data_ptr(), ent.data_ptr(),
+                          stat.data_ptr(), _p(tl), _p(ti), top, rows, V, _st())
+        ctx.save_for_backward(x, t, stat)
+        ctx.cfg = (logits.shape, ignore_index)
+        ctx.set_materialize_grads(False)
+        if top:
+            tl, ti = tl.view(*shp, top), ti.view(*shp, top)
+            ctx.mark_non_differentiable(tl, ti)
+        return logp.view(shp), ent.view(shp), tl, ti
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogp, dent, *_):
+        x, t, stat = ctx.saved_tensors
+        shape, ignore_index = ctx.cfg
+        rows, V = x.shape
+        # the gradient's rows start where the logits' rows do, so that both move in whole vectors; a wide gap between rows is not repeated
+        ld = x.stride(0) if x.stride(0) < V + 64 else V
+        dx = torch.empty((rows, ld), dtype=x.dtype, device=x.device)[:, :V]
+        g = None if dlogp is None else dlogp.reshape(-1).float().contiguous()
+        h = None if dent is None else dent.reshape(-1).float().contiguous()
+        if rows:
+            with torch.cuda.device(x.device):
+                _lib.call("vlni_token_logprobs_bwd", _dt(x), _p(g), _p(h), x.data_ptr(), x.stride(0), t.data_ptr(), ignore_index, stat.data_ptr(),
+                          dx.data_ptr(), ld, rows, V, _st())
+        return dx.view(shape) if ld == V else dx.unflatten(0, shape[:-1]), None, None, None
+
+
+def token_logprobs(logits, target, top=0, ignore_index=-100):
+    """Log probability of `target` under softmax(logits), the entropy of every row, and its `top` most likely alternatives.
+
+    logits [..., V] float32, bfloat16 or float16 (may hold -inf: impossible actions); target int64 [...]. Returns (logp, entropy, top_logp, top_index):
+    float32 [...], float32 [...], float32 and int64 [..., top] (None with top = 0), the alternatives in falling order, equal ones by lowest index.
+    logp and entropy are differentiable (policy gradient with entropy bonus, r2r/agent_cmt.py:569-574,702-744; masked-token losses), the alternatives
+    are not. A target equal to ignore_index, or outside [0, V), has logp 0 and sends no gradient through it; the latter are counted
+    (`watch_index_errors` / `index_errors`). A row of -inf only: logp -inf, entropy 0, no gradient. top <= 16."""
+    _dt(logits)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"token_logprobs: logits {tuple(logits.shape)}")
+    if target.dtype != torch.int64 or target.shape != logits.shape[:-1]:
+        raise ValueError(f"token_logprobs: target is {target.dtype} {tuple(target.shape)}, expected int64 {tuple(logits.shape[:-1])}")
+    if not 0 <= top <= min(16, logits.shape[-1]):
+        raise ValueError(f"token_logprobs: top = {top} of {logits.shape[-1]} (at most 16)")
+    if logits.shape[-1] >= 1 << 30:
+        raise ValueError(f"token_logprobs: {logits.shape[-1]} columns")
+    _same_device(logits, "logits", target=target)
+    return _TokenLogprobs.apply(logits, target, int(top), int(ignore_index))
