@@ -19,8 +19,9 @@ struct LaP {
   const float* bvec;           // [nh, BL] bias by distance in units of log2, saturated LA_PAD beyond +-R; null without a bias
   float* part; float* part_ml; // split launches: float32 partial results; running (maximum, sum)
   void *dq, *dk, *dv;
-  float* dbpart;               // [nh][B * row blocks * splits][BL] sums of dS by distance, or null
-  int B, Sq, Sk, SkP, nh, nkv, D, causal, PG, R, BL, nblk, nsplit;
+  float* rowsum;               // [splits][5][B, nh, Sq] sums of a row's dS and P (see la_dq_kernel), null without a table gradient
+  float* dbpart;               // [nh][B * row blocks][BL] sums of dS by distance
+  int B, Sq, Sk, SkP, nh, nkv, D, causal, PG, R, BL, nblk, nsplit, zrow;
   float c1, scale;             // c1 = scale log2(e)
 };
 

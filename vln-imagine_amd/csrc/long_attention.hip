@@ -129,18 +129,20 @@ void la_prep_pointers(const VlniLongAttnArgs* a, LaP& p) {
   }
   if (a->rel_table) p.bvec = f;
 }
-// floats of workspace: forward: split results; backward: delta, sums by distance, split results (of dQ, then of dK and dV)
+// floats of workspace: forward: split results; backward: delta, row sums, sums by distance, split results (of dQ, then of dK and dV)
 long la_fwd_work(const VlniLongAttnArgs* a, LaP p) {
   la_grid_rows(a, p);
   const long n = (long)p.B * p.Sq * p.nh;
   return p.nsplit > 1 ? p.nsplit * n * (p.D + 2) : 0;
 }
-long la_bwd_work(const VlniLongAttnArgs* a, LaP p, long* o_db, long* o_part) {
+long la_bwd_work(const VlniLongAttnArgs* a, LaP p, long* o_rs, long* o_db, long* o_part) {
   const long n = (long)p.B * p.Sq * p.nh;
   long f = (n + 3) & ~3L;
   la_grid_rows(a, p);
+  *o_rs = f;
+  if (a->rel_table) f += 5 * p.nsplit * n;
   *o_db = f;
-  if (a->rel_table) f += (long)p.nh * p.B * p.nblk * p.nsplit * p.BL;
+  if (a->rel_table) f += (long)p.nh * p.B * p.nblk * p.BL;
   f = (f + 3) & ~3L;
   *o_part = f;
   long part = p.nsplit > 1 ? p.nsplit * n * p.D : 0;
@@ -170,10 +172,10 @@ int la_go(const VlniLongAttnArgs* a, const LaP& p, int what, hipStream_t st) {
 extern "C" int vlni_long_attn_sizes(const VlniLongAttnArgs* a, long* sizes) {
   LaP p; LaBuckets k;
   LA_TRY(la_fill(a, p, k));
-  long o1, o2;
+  long o1, o2, o3;
   sizes[0] = la_prep_floats(a, p);
   sizes[1] = la_fwd_work(a, p);
-  sizes[2] = la_bwd_work(a, p, &o1, &o2);
+  sizes[2] = la_bwd_work(a, p, &o1, &o2, &o3);
   return VLNI_OK;
 }
 
@@ -221,8 +223,8 @@ extern "C" int vlni_long_attn_bwd(const VlniLongAttnArgs* a, void* stream) {
              a->dq, a->dk, a->dv);
   VLNI_CHECK(!a->dtable || a->rel_table, VLNI_EINVAL, "long_attn: a table gradient without a table");
   const long n = (long)p.B * p.Sq * p.nh, need = la_prep_floats(a, p);
-  long o_db, o_part;
-  const long work = la_bwd_work(a, p, &o_db, &o_part);
+  long o_rs, o_db, o_part;
+  const long work = la_bwd_work(a, p, &o_rs, &o_db, &o_part);
   VLNI_CHECK(!need || (a->prep && a->prep_floats >= need), VLNI_EINVAL, "long_attn: prep holds %ld floats, %ld are needed", a->prep ? a->prep_floats : 0, need);
   VLNI_CHECK(a->work && a->work_floats >= work && (uintptr_t)a->work % 16 == 0, VLNI_EINVAL, "long_attn: work holds %ld floats, %ld are needed",
              a->work ? a->work_floats : 0, work);
@@ -237,12 +239,13 @@ extern "C" int vlni_long_attn_bwd(const VlniLongAttnArgs* a, void* stream) {
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   float* f = (float*)a->work;
   p.delta = f;
-  p.dbpart = a->dtable ? f + o_db : nullptr;
+  p.rowsum = a->dtable ? f + o_rs : nullptr;
+  p.dbpart = f + o_db;
   p.part = f + o_part;
   la_grid_rows(a, p);
   LA_TRY(la_go(a, p, 1, st));
   if (a->dtable) {
-    hipLaunchKernelGGL(la_dtable_kernel, dim3(k.n * k.sides, p.nh), dim3(256), 0, st, p.dbpart, a->dtable, k, p.nh, p.R, p.BL, p.B * p.nblk * p.nsplit);
+    hipLaunchKernelGGL(la_dtable_kernel, dim3(k.n * k.sides, p.nh), dim3(256), 0, st, p.dbpart, a->dtable, k, p.nh, p.R, p.BL, p.B * p.nblk);
     VLNI_LAUNCH_CHECK();
   }
   la_grid_keys(a, p);
