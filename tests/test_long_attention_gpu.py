@@ -6,7 +6,8 @@ Bounds are elementwise and follow from the arithmetic, with u = eps / 2 of the 1
   out      (u + epsP + n 2^-24) P|V| + u |out|            (P rounded once, out rounded once)
   delta    |dO| . (error of out) + D 2^-24 |dO|.|out|
   dS       u |dS| + epsP |dS| + P (error of delta + D 2^-24 |dO|.|V|)
-  dV, dQ, dK   the same sums over the errors of P and dS, and one rounding of the result; the table's gradient sums dS before it is rounded.
+  dV, dQ, dK   the same sums over the errors of P and dS, and one rounding of the result; the table's gradient sums dS before it is rounded
+           and with delta from the rows' own sums.
 float16 adds half its smallest step (2^-25) wherever a P, a dS or a result below its normal range is rounded."""
 import math
 
@@ -92,6 +93,9 @@ def _reference(q, k, v, dout, kmask, causal, scale, table, rel_max, bidir):
         res[n] = (g, e + u * g.abs())
     res = {n: (a.transpose(1, 2), b.transpose(1, 2) + tiny + 1e-30) for n, (a, b) in res.items()}
     if table is not None:
+        # the table's gradient takes every row's delta from the sum of its dS, not from the rounded out: no error of out in it
+        row = ((epsP + nk) * (aS + P * edelta)).sum(-1, keepdim=True)
+        eS = epsP * aS + P * (row + D * e24 * (dO.abs() @ V.abs().transpose(2, 3)) + 4 * e24 * (dP.abs() + delta.abs()))
         gt, et = torch.zeros_like(table, dtype=torch.float64), torch.zeros_like(table, dtype=torch.float64)
         for b in range(table.shape[0]):
             w = (which == b)

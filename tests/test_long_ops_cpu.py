@@ -8,6 +8,25 @@ import torch
 from vln_imagine_amd import _lib, ops
 
 
+class Args(ctypes.Structure):                # VlniLongAttnArgs (include/vlni.h)
+    _fields_ = [(n, ctypes.c_int) for n in ("dtype", "B", "Sq", "Sk", "nh", "nkv", "D", "causal")] + \
+               [("scale", ctypes.c_float), ("rel_n", ctypes.c_int), ("rel_sides", ctypes.c_int), ("rel_first", ctypes.c_void_p)] + \
+               [(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout")] + \
+               [(n, ctypes.c_long * 3) for n in ("q_stride", "k_stride", "v_stride", "do_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("kmask", "rel_table", "out", "stat")] + \
+               [("prep", ctypes.c_void_p), ("prep_floats", ctypes.c_long), ("work", ctypes.c_void_p), ("work_floats", ctypes.c_long)] + \
+               [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "dtable")]
+
+
+def test_packed_arguments_have_the_structures_layout():
+    assert ops._LA_ARGS.size == ctypes.sizeof(Args)
+    vals = list(range(1, 9)) + [0.5] + list(range(10, 41))
+    a = Args.from_buffer_copy(ops._LA_ARGS.pack(*vals))
+    assert (a.dtype, a.causal, a.scale, a.rel_sides, a.rel_first, a.q, a.dout) == (1, 8, 0.5, 11, 12, 13, 16)
+    assert list(a.q_stride) == [17, 18, 19] and list(a.do_stride) == [26, 27, 28]
+    assert (a.kmask, a.rel_table, a.out, a.stat, a.prep, a.prep_floats, a.work, a.work_floats, a.dq, a.dtable) == (29, 30, 31, 32, 33, 34, 35, 36, 37, 40)
+
+
 def _qkv(B=2, Sq=5, Sk=7, nh=4, nkv=2, D=64, dtype=torch.float32):
     return torch.zeros(B, Sq, nh, D, dtype=dtype), torch.zeros(B, Sk, nkv, D, dtype=dtype), torch.zeros(B, Sk, nkv, D, dtype=dtype)
 
@@ -50,7 +69,7 @@ def test_c_entry_points_refuse():
     lib = _lib.load()
 
     def args(**kw):
-        a = ops._LongAttnArgs()
+        a = Args()
         a.dtype, a.B, a.Sq, a.Sk, a.nh, a.nkv, a.D, a.scale = 1, 2, 5, 7, 4, 2, 64, 0.125
         for n in ("q", "k", "v", "dout", "out", "stat", "work", "dq", "dk", "dv"):
             setattr(a, n, 4096)

@@ -15,7 +15,7 @@ struct LaP {
   float* lse; float* rl;       // [B, nh, Sq] each: see the masks' comment above
   float* delta;                // [B, nh, Sq]
   const float* kml;            // [B, SkP] mask in units of log2, -inf behind Sk; null without a mask
-  const int* kind;             // [B, SkP / 64]: 0 no mask in these 64 keys, 1 some, 2 nothing but -inf
+  const int* kind;             // [B, SkP / 64]: 0 no mask in these 64 keys, 1 finite values, 2 nothing but -inf, 3 some -inf
   const float* bvec;           // [nh, BL] bias by distance in units of log2, saturated LA_PAD beyond +-R; null without a bias
   float* part; float* part_ml; // split launches: float32 partial results; running (maximum, sum)
   void *dq, *dk, *dv;

@@ -34,8 +34,8 @@ __global__ __launch_bounds__(64) void la_prep_kernel(const float* kmask, const f
       if (v != -INFINITY) v = (v < LA_LOWEST ? LA_LOWEST : v) * LA_LOG2E;      // (NaN and +inf stay)
     }
     kml[(long)b * SkP + j] = v;
-    const bool none = __all(v == 0.f), all = __all(v == -INFINITY);
-    if (lane == 0) kind[blockIdx.x] = none ? 0 : all ? 2 : 1;
+    const bool none = __all(v == 0.f), all = __all(v == -INFINITY), some = __any(v == -INFINITY);
+    if (lane == 0) kind[blockIdx.x] = none ? 0 : all ? 2 : some ? 3 : 1;
   } else {
     const int per = (BL + 63) / 64, w = blockIdx.x - nmask, h = w / per, e = (w % per) * 64 + lane;
     if (e >= BL) return;

@@ -11,6 +11,7 @@ sequence with fused epilogues (bias, GELU / GELU', residual) instead of ~40 tiny
 import bisect
 import ctypes
 import os
+import struct
 import weakref
 
 import numpy as np
@@ -3529,14 +3530,8 @@ def cosine(x, y):
 # =====================================================================================
 #  attention over long sequences, token log probabilities
 # =====================================================================================
-class _LongAttnArgs(ctypes.Structure):       # VlniLongAttnArgs (include/vlni.h)
-    _fields_ = [(n, ctypes.c_int) for n in ("dtype", "B", "Sq", "Sk", "nh", "nkv", "D", "causal")] + \
-               [("scale", ctypes.c_float), ("rel_n", ctypes.c_int), ("rel_sides", ctypes.c_int), ("rel_first", ctypes.c_void_p)] + \
-               [(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout")] + \
-               [(n, ctypes.c_long * 3) for n in ("q_stride", "k_stride", "v_stride", "do_stride")] + \
-               [(n, ctypes.c_void_p) for n in ("kmask", "rel_table", "out", "stat")] + \
-               [("prep", ctypes.c_void_p), ("prep_floats", ctypes.c_long), ("work", ctypes.c_void_p), ("work_floats", ctypes.c_long)] + \
-               [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "dtable")]
+# VlniLongAttnArgs (include/vlni.h), packed in one go: filling a ctypes structure field by field costs more than launching a kernel
+_LA_ARGS = struct.Struct("@8ifiiP4P12l4PPlPl4P")
 
 
 _REL_FIRST = {}
@@ -3559,19 +3554,43 @@ def rel_bucket_starts(n, rel_max):
 
 
 def _la_view(t):
-    """t itself where the kernels can read it (the last axis contiguous, everything else on 16-byte steps), else a dense copy."""
-    step = 16 // t.element_size()
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] == 1 or (t.stride(i) % step == 0 and t.stride(i) >= 0) for i in range(3))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    """(t, its strides of sample, position and head) where the kernels can read it: the last axis contiguous, everything else on 16-byte steps; else of a
+    dense copy."""
+    st, step = t.stride(), 16 // t.element_size() - 1
+    if st[3] == 1 and not (st[0] | st[1] | st[2]) & step and not t.data_ptr() & 15:
+        return t, st[:3]
+    sh = t.shape
+    st = tuple(0 if sh[i] == 1 else st[i] for i in range(3)) + (1 if sh[3] == 1 else st[3],)       # an axis of one element may claim any stride
+    if st[3] != 1 or (st[0] | st[1] | st[2]) & step or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = t.stride()
+    return t, st[:3]
 
 
-def _la_strides(t):
-    return (ctypes.c_long * 3)(*[t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)])
+_LA_SIZES = {}
 
 
-def _la_call(fn, a, device):
-    with torch.cuda.device(device):
-        _lib.call(fn, ctypes.addressof(a), _st())
+def _la_sizes(head, masked, biased):
+    """(floats of prep, of the forward's work, of the backward's work) for one set of shapes."""
+    key = (*head, masked, biased)
+    n = _LA_SIZES.get(key)
+    if n is None:
+        sizes = (ctypes.c_long * 3)()
+        # (of the pointers only the presence of mask and table matters here)
+        _lib.call("vlni_long_attn_sizes", _LA_ARGS.pack(*head, *[0] * 16, int(masked), int(biased), *[0] * 10), ctypes.addressof(sizes))
+        if len(_LA_SIZES) >= 4096:
+            _LA_SIZES.clear()
+        n = _LA_SIZES[key] = tuple(sizes)
+    return n
+
+
+def _call_on(dev, fn, *args):
+    """On torch's current stream of the tensors' device, whichever device is current."""
+    if dev == torch.cuda.current_device():
+        _lib.call(fn, *args, _st())
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(fn, *args, _st())
 
 
 class _LongAttention(torch.autograd.Function):
@@ -3579,66 +3598,64 @@ class _LongAttention(torch.autograd.Function):
     backward pass recomputes the probabilities. Inside an EpisodeTape it computes in every pass, the ghost pass included (on the filled buffers)."""
 
     @staticmethod
-    def _args(q, k, v, kmask, table, cfg):
-        causal, scale, sides, first = cfg
-        a = _LongAttnArgs()
-        a.dtype, a.B, a.Sq, a.nh, a.D = _dt(q), *q.shape
-        a.Sk, a.nkv, a.causal, a.scale = k.shape[1], k.shape[2], int(causal), scale
-        a.q, a.k, a.v, a.kmask, a.rel_table = q.data_ptr(), k.data_ptr(), v.data_ptr(), _p(kmask), _p(table)
-        a.q_stride, a.k_stride, a.v_stride = _la_strides(q), _la_strides(k), _la_strides(v)
-        if table is not None:
-            a.rel_n, a.rel_sides, a.rel_first = len(first), sides, ctypes.addressof(first)
-        sizes = (ctypes.c_long * 3)()
-        _lib.call("vlni_long_attn_sizes", ctypes.addressof(a), ctypes.addressof(sizes))
-        return a, sizes
-
-    @staticmethod
-    def forward(ctx, q, k, v, kmask, table, cfg):
-        ctx.cfg, ctx.shapes = cfg, (q.shape, k.shape)
-        ctx.empty = q.numel() == 0 or k.numel() == 0
-        if ctx.empty:
-            ctx.tshape = None if table is None else table.shape
+    def forward(ctx, q, k, v, kmask, table, causal, scale, sides, first):
+        ctx.set_materialize_grads(False)
+        if q.numel() == 0 or k.numel() == 0:
+            ctx.head = None
+            ctx.save_for_backward(q, k, v, table)
             return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        q, k, v = _la_view(q), _la_view(k), _la_view(v)
+        (B, Sq, nh, D), dev = q.shape, q.get_device()
+        (q, qs), (k, ks), (v, vs) = _la_view(q), _la_view(k), _la_view(v)
         kmask = None if kmask is None else kmask.contiguous()
         table = None if table is None else table.contiguous()
-        a, sizes = _LongAttention._args(q, k, v, kmask, table, cfg)
-        B, Sq, nh, D = q.shape
-        out = torch.empty((B, Sq, nh, D), dtype=q.dtype, device=q.device)
-        stat = torch.empty((2, B, nh, Sq), dtype=torch.float32, device=q.device)
-        prep = torch.empty((sizes[0],), dtype=torch.float32, device=q.device) if sizes[0] else None
-        work = torch.empty((sizes[1],), dtype=torch.float32, device=q.device) if sizes[1] else None
-        a.out, a.stat, a.prep, a.prep_floats, a.work, a.work_floats = out.data_ptr(), stat.data_ptr(), _p(prep), sizes[0], _p(work), sizes[1]
-        _la_call("vlni_long_attn_fwd", a, q.device)
-        ctx.save_for_backward(q, k, v, kmask, table, out, stat, prep)
+        n = 0 if first is None else len(first)
+        Sk, nkv = k.shape[1], k.shape[2]
+        head = (_dt(q), B, Sq, Sk, nh, nkv, D, causal, scale, n, sides, 0 if first is None else ctypes.addressof(first))
+        n_prep, n_fwd, n_bwd = _la_sizes(head, kmask is not None, table is not None)
+        out = q.new_empty((B, Sq, nh, D))
+        keep = torch.empty((2 * B * nh * Sq + n_prep,), dtype=torch.float32, device=q.device)          # stat, then prep
+        work = torch.empty((n_fwd,), dtype=torch.float32, device=q.device) if n_fwd else None
+        stat = keep.data_ptr()
+        mid = (*qs, *ks, *vs)
+        ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr())
+        tail = (_p(kmask), _p(table), out.data_ptr(), stat, stat + 8 * B * nh * Sq, n_prep)
+        _call_on(dev, "vlni_long_attn_fwd", _LA_ARGS.pack(*head, *ptrs, 0, *mid, 0, 0, 0, *tail, _p(work), n_fwd, 0, 0, 0, 0))
+        ctx.save_for_backward(q, k, v, kmask, table, out, keep)
+        ctx.head, ctx.first, ctx.mid, ctx.tail, ctx.n_bwd = head, first, mid, tail, n_bwd
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
+    def _backward(ctx, dout):
         ng = ctx.needs_input_grad
-        qs, ks = ctx.shapes
-        if ctx.empty:
-            z = [torch.zeros(s, dtype=dout.dtype, device=dout.device) if n else None for s, n in zip((qs, ks, ks), ng)]
-            return (*z, None, torch.zeros(ctx.tshape, dtype=torch.float32, device=dout.device) if ng[4] else None, None)
-        q, k, v, kmask, table, out, stat, prep = ctx.saved_tensors
-        dout = _la_view(dout)
-        a, sizes = _LongAttention._args(q, k, v, kmask, table, ctx.cfg)
-        dq = torch.empty(qs, dtype=q.dtype, device=q.device)
-        dk, dv = (torch.empty(ks, dtype=q.dtype, device=q.device) for _ in range(2))
+        if dout is None:
+            return (None,) * 9
+        if ctx.head is None:
+            return (*[torch.zeros(t.shape, dtype=t.dtype, device=t.device) if n and t is not None else None
+                      for t, n in zip(ctx.saved_tensors[:3] + (None, ctx.saved_tensors[3]), ng)], None, None, None, None)
+        q, k, v, kmask, table, out, keep = ctx.saved_tensors
+        dout, ds = _la_view(dout)
+        dq, dk, dv = q.new_empty(out.shape), q.new_empty(k.shape), q.new_empty(k.shape)
         dtable = torch.empty_like(table) if ng[4] else None
-        work = torch.empty((sizes[2],), dtype=torch.float32, device=q.device)
-        a.dout, a.do_stride = dout.data_ptr(), _la_strides(dout)
-        a.out, a.stat, a.prep, a.prep_floats, a.work, a.work_floats = out.data_ptr(), stat.data_ptr(), _p(prep), sizes[0], work.data_ptr(), sizes[2]
-        a.dq, a.dk, a.dv, a.dtable = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(dtable)
-        _la_call("vlni_long_attn_bwd", a, q.device)
-        return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, None, dtable, None
+        work = torch.empty((ctx.n_bwd,), dtype=torch.float32, device=q.device)
+        args = _LA_ARGS.pack(*ctx.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *ctx.mid, *ds, *ctx.tail, work.data_ptr(), ctx.n_bwd,
+                             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(dtable))
+        _call_on(q.get_device(), "vlni_long_attn_bwd", args)
+        return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, None, dtable, None, None, None, None
+
+    @staticmethod
+    def backward(ctx, dout):
+        # (once_differentiable's bookkeeping is only needed where a second derivative may be asked for)
+        return _LongAttention._once(ctx, dout) if torch.is_grad_enabled() else _LongAttention._backward(ctx, dout)
+
+
+_LongAttention._once = staticmethod(torch.autograd.function.once_differentiable(_LongAttention._backward))
 
 
 def _same_device(t0, name0, **others):
     _chk(t0, name0)
+    dev = t0.device
     for n, t in others.items():
-        if t is not None and t.device != t0.device:
+        if t is not None and t.device != dev:
             raise RuntimeError(f"vlni: {n} is on {t.device}, {name0} on {t0.device}")
 
 
@@ -3687,7 +3704,7 @@ def long_attention(q, k, v, kmask=None, causal=False, scale=None, rel_table=None
             raise ValueError(f"long_attention: rel_max {rel_max} with {n} buckets a side: a whole number above {n // 2}, at most 1024")
         first = rel_bucket_starts(n, int(rel_max))
     _same_device(q, "q", k=k, v=v, kmask=kmask, rel_table=rel_table)
-    return _LongAttention.apply(q, k, v, kmask, rel_table, (bool(causal), scale, sides, first))
+    return _LongAttention.apply(q, k, v, kmask, rel_table, int(bool(causal)), scale, sides, first)
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -3695,42 +3712,50 @@ class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, target, top, ignore_index):
-        shp, V = logits.shape[:-1], logits.shape[-1]
-        x = _rows(logits)
+        shape = logits.shape
+        shp, V = shape[:-1], shape[-1]
+        x, t = _rows(logits), target.contiguous()
         rows, dev = x.shape[0], x.device
-        t = target.reshape(-1).contiguous()
-        logp, ent = (torch.empty((rows,), dtype=torch.float32, device=dev) for _ in range(2))
-        stat = torch.empty((rows, 3), dtype=torch.float32, device=dev)
-        tl = torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None
-        ti = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
-        if rows:
-            with torch.cuda.device(dev):
-                _lib.call("vlni_token_logprobs_fwd", _dt(x), x.data_ptr(), x.stride(0), t.data_ptr(), ignore_index, logp.data_ptr(), ent.data_ptr(),
-                          stat.data_ptr(), _p(tl), _p(ti), top, rows, V, _st())
-        ctx.save_for_backward(x, t, stat)
-        ctx.cfg = (logits.shape, ignore_index)
-        ctx.set_materialize_grads(False)
+        logp, ent = torch.empty(shp, dtype=torch.float32, device=dev), torch.empty(shp, dtype=torch.float32, device=dev)
+        stat = torch.empty((3 * rows,), dtype=torch.float32, device=dev)
+        tl = ti = None
         if top:
-            tl, ti = tl.view(*shp, top), ti.view(*shp, top)
+            tl, ti = torch.empty((*shp, top), dtype=torch.float32, device=dev), torch.empty((*shp, top), dtype=torch.int64, device=dev)
             ctx.mark_non_differentiable(tl, ti)
-        return logp.view(shp), ent.view(shp), tl, ti
+        if rows:
+            _call_on(x.get_device(), "vlni_token_logprobs_fwd", _dt(x), x.data_ptr(), x.stride(0), t.data_ptr(), ignore_index, logp.data_ptr(), ent.data_ptr(),
+                     stat.data_ptr(), _p(tl), _p(ti), top, rows, V)
+        ctx.save_for_backward(x, t, stat)
+        ctx.cfg = (shape, ignore_index)
+        ctx.set_materialize_grads(False)
+        return logp, ent, tl, ti
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dlogp, dent, *_):
+    def _backward(ctx, dlogp, dent, *_):
         x, t, stat = ctx.saved_tensors
         shape, ignore_index = ctx.cfg
+        if dlogp is None and dent is None:
+            return None, None, None, None
         rows, V = x.shape
         # the gradient's rows start where the logits' rows do, so that both move in whole vectors; a wide gap between rows is not repeated
         ld = x.stride(0) if x.stride(0) < V + 64 else V
-        dx = torch.empty((rows, ld), dtype=x.dtype, device=x.device)[:, :V]
-        g = None if dlogp is None else dlogp.reshape(-1).float().contiguous()
-        h = None if dent is None else dent.reshape(-1).float().contiguous()
+        g = None if dlogp is None else dlogp.float().contiguous()
+        h = None if dent is None else dent.float().contiguous()
+        if ld == V:
+            dx = x.new_empty(shape)
+        else:
+            dx = x.new_empty((*shape[:-1], ld))[..., :V]
         if rows:
-            with torch.cuda.device(x.device):
-                _lib.call("vlni_token_logprobs_bwd", _dt(x), _p(g), _p(h), x.data_ptr(), x.stride(0), t.data_ptr(), ignore_index, stat.data_ptr(),
-                          dx.data_ptr(), ld, rows, V, _st())
-        return dx.view(shape) if ld == V else dx.unflatten(0, shape[:-1]), None, None, None
+            _call_on(x.get_device(), "vlni_token_logprobs_bwd", _dt(x), _p(g), _p(h), x.data_ptr(), x.stride(0), t.data_ptr(), ignore_index, stat.data_ptr(),
+                     dx.data_ptr(), ld, rows, V)
+        return dx, None, None, None
+
+    @staticmethod
+    def backward(ctx, *g):
+        return _TokenLogprobs._once(ctx, *g) if torch.is_grad_enabled() else _TokenLogprobs._backward(ctx, *g)
+
+
+_TokenLogprobs._once = staticmethod(torch.autograd.function.once_differentiable(_TokenLogprobs._backward))
 
 
 def token_logprobs(logits, target, top=0, ignore_index=-100):
