@@ -44,7 +44,8 @@ __global__ __launch_bounds__(64) void la_prep_kernel(const float* kmask, const f
   }
 }
 
-// dtable[bucket][head] = sum of dS over the bucket's distances and all partial rows of the head; block = one (bucket, head), fixed order
+// dtable[bucket][head] = sum of dS over the bucket's distances and all partial rows of the head; block = one (bucket, head), 8 rows x 32 distances at a
+// time, in a fixed order and in 64 bits
 __global__ __launch_bounds__(256) void la_dtable_kernel(const float* part, float* dtable, LaBuckets k, int nh, int R, int BL, int nparts) {
   const int b = blockIdx.x, h = blockIdx.y, side = b / k.n, bb = b % k.n;
   const int d0 = k.first[bb], d1 = bb + 1 < k.n ? k.first[bb + 1] - 1 : INT_MAX;       // distances d0 .. d1 (none: d1 < d0)
@@ -57,10 +58,9 @@ __global__ __launch_bounds__(256) void la_dtable_kernel(const float* part, float
     e1 = k.sides == 1 && d0 == 0 && d1 >= 0 ? BL - 1 : R + LA_PAD - d0;
   }
   double a = 0.0;
-  const int n = e1 - e0 + 1;
-  if (n > 0) {
-    const long total = (long)nparts * n;
-    for (long x = threadIdx.x; x < total; x += 256) a += (double)part[((long)h * nparts + x / n) * BL + e0 + x % n];
+  for (int q = threadIdx.x >> 5; q < nparts; q += 8) {
+    const float* row = part + ((long)h * nparts + q) * BL;
+    for (int e = e0 + (threadIdx.x & 31); e <= e1; e += 32) a += (double)row[e];
   }
   __shared__ double s[256];
   s[threadIdx.x] = a;
@@ -101,21 +101,35 @@ int la_fill(const VlniLongAttnArgs* a, LaP& p, LaBuckets& k) {
   return VLNI_OK;
 }
 
-// launches below a full chip are split along their loop: enough blocks for two per CU, at least two tiles each
-int la_split(long blocks, long tiles) {
-  if (blocks >= 256 || tiles < 4) return 1;
-  const long want = (512 + blocks - 1) / blocks;
-  const long most = tiles / 2;
-  return (int)(want < most ? want : most);
+// Splits of a launch along its loop: the chip works through `tiles` tiles in all at `us` microseconds a tile and CU, but no faster than the longest block
+// (`chain` tiles), whose end it partly waits for; splits shorten that and cost their partial results (float32, written and read at 4 TB/s) and a launch.
+// Measured: dK / dV of a causal 4 k pass with four key heads, 256 blocks: 301 us whole, 190 us in four.
+int la_split(double tiles, double chain, double us, double floats) {
+  int best = 1;
+  double least = 1e300;
+  for (int n = 1; n <= 32 && (n == 1 || chain / n >= 2.0); ++n) {
+    const double all = tiles / 256.0, one = chain / n;
+    const double t = us * (one > all + 0.5 * one ? one : all + 0.5 * one) + (n > 1 ? 6.0 + n * floats * 8.0 / 4e6 : 0.0);
+    if (t < 0.98 * least) { best = n; least = t; }
+  }
+  return best;
 }
 int la_kt_of(const VlniLongAttnArgs* a) { return a->dtype == VLNI_F32 && a->D > 64 ? 32 : 64; }
+// microseconds of a 64 x 128 tile on a CU: measured at D = 64, 16 bit; float32 products run at a tenth of the rate
+double la_tile_us(const VlniLongAttnArgs* a, double us) {
+  return us * ((a->D + 31) / 32 * 32) / 64.0 * la_kt_of(a) / 64.0 * (a->dtype == VLNI_F32 ? 7.0 : 1.0);
+}
 void la_grid_rows(const VlniLongAttnArgs* a, LaP& p) {
   p.nblk = cdiv((long)p.Sq * p.PG, 128);
-  p.nsplit = la_split((long)p.nblk * p.B * (p.nh / p.PG), cdiv(p.Sk, la_kt_of(a)));
+  const double chain = cdiv(p.Sk, la_kt_of(a)), blocks = (double)p.nblk * p.B * (p.nh / p.PG);
+  const double part = p.causal && p.PG == 1 ? (p.Sk - 0.5 * (p.Sq < p.Sk ? p.Sq : p.Sk)) / p.Sk : 1.0;
+  p.nsplit = la_split(blocks * chain * part, chain, la_tile_us(a, 0.9), (double)p.B * p.Sq * p.nh * p.D);
 }
 void la_grid_keys(const VlniLongAttnArgs* a, LaP& p) {
   p.nblk = cdiv(p.Sk, 128);
-  p.nsplit = la_split((long)p.nblk * p.B * p.nkv, (long)cdiv((long)p.Sq * p.PG, la_kt_of(a)) * (p.nh / p.nkv / p.PG));
+  const double chain = (double)cdiv((long)p.Sq * p.PG, la_kt_of(a)) * (p.nh / p.nkv / p.PG), blocks = (double)p.nblk * p.B * p.nkv;
+  const double part = p.causal && p.PG == 1 ? (p.Sk - 0.5 * (p.Sq < p.Sk ? p.Sq : p.Sk)) / p.Sk : 1.0;
+  p.nsplit = la_split(blocks * chain * part, chain, la_tile_us(a, 1.6), 2.0 * p.B * p.Sk * p.nkv * p.D);
 }
 long la_prep_floats(const VlniLongAttnArgs* a, const LaP& p) {
   return (a->kmask ? (long)p.B * p.SkP + (long)p.B * (p.SkP >> 6) : 0) + (a->rel_table ? (long)p.nh * p.BL : 0);
