@@ -7,14 +7,21 @@
 // them once and writes the gradient; nothing else of the logits' size is made. Rows start at any element (30522 16-bit columns are no multiple
 // of 16 bytes): vectors are laid on the row's 16-byte boundaries, and the partial ones at its ends are read and written element by element.
 //
-// Alternatives: a row (or 32 k of it at a time) sits in registers, so the best is taken out `top` times; a 64-bit key (order-preserving bits of
-// x, then the complement of the index) makes "largest value, lowest index" one comparison. Only the wave that lost its best looks again.
+// Alternatives: the row's threads form 16 groups; the top-th largest of the groups' maxima is a lower bound of the top-th largest element, so only
+// elements not below it (a dozen on ordinary logits) are candidates. They meet in LDS as 64-bit keys (order-preserving bits of x, then the
+// complement of the index: one comparison means "larger value, then lower index") and are ranked by counting. Where ties make more than 48 of them, the
+// best is taken out `top` times instead.
+#include <limits.h>
+
 #include "../../include/vlni.h"
 #include "common.h"
 
 namespace {
 
-constexpr int LP_MAXTOP = 16;
+constexpr int LP_MAXTOP = 16, LP_MANY = 1024;
+#ifndef LP_WPE
+#define LP_WPE 4
+#endif
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 typedef unsigned long long u64;
 
@@ -75,31 +82,76 @@ template <typename T, int VEC> __device__ __forceinline__ void lp_load(float (&x
 template <typename T> __device__ __forceinline__ int lp_head(const T* row) {      // elements between the 16-byte boundary below the row and the row
   return (int)(((uintptr_t)row & 15) / sizeof(T));
 }
+// the threads of a row: a wave (its LDS operations are in order: nothing but the compiler has to be held) or the block
+template <int NW> __device__ __forceinline__ void lp_sync() {
+  if constexpr (NW == 1) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+
+constexpr int LP_CAND = 48;
+struct LpTop {
+  u64 list[16], cand[LP_CAND], wbest[16];
+  float gmax[16];
+  int count;
+};
 
 // TPB threads per row (64: four rows a block), N vectors of VEC elements a thread and pass
-template <typename T, int TPB, int VEC, int N, bool TOP>
-__global__ __launch_bounds__(TPB < 256 ? 256 : TPB) void lp_fwd_kernel(LpP p) {
-  constexpr int NW = TPB / 64;                       // waves of a row
-  __shared__ u64 wbest[16];
+template <typename T, int TPB, int VEC, int N, bool TOP, int WPE>
+__global__ __launch_bounds__(TPB < 256 ? 256 : TPB, WPE) void lp_fwd_kernel(LpP p) {
+  constexpr int NW = TPB / 64, RPB = TPB < 256 ? 256 / TPB : 1, GL = TPB / 16;       // waves and rows, threads of a group
+  __shared__ LpTop tops[TOP ? RPB : 1];
   __shared__ float red[3][16];
   const int tid = threadIdx.x % TPB, lane = threadIdx.x & 63, wave = NW == 1 ? 0 : tid >> 6;
   const long row_i = NW == 1 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (NW == 1 && row_i >= p.rows) return;
+  LpTop& q = tops[TOP && NW == 1 ? threadIdx.x >> 6 : 0];
   const T* row = (const T*)p.x + row_i * p.ld;
-  const long e0 = VEC == 1 ? 0 : -lp_head(row);
+  // whole vectors [first, first + full VEC), up to VEC - 1 elements on either side of them: one more element for the first 2 VEC threads
+  const int first = VEC == 1 ? 0 : (VEC - lp_head(row)) % VEC, full = VEC == 1 ? p.V : (p.V - first) / VEC;
   float m = -INFINITY, l = 0.f, s = 0.f;
-  u64 list = 0;                                      // lane q of every wave: the q-th best so far
-  for (long c0 = e0; c0 < p.V; c0 += (long)TPB * N * VEC) {
-    float x[N][VEC];
+  if (TOP) {
+    if (tid < 16) q.list[tid] = 0;
+    if (tid == 0) q.count = 0;
+    lp_sync<NW>();
+  }
+  for (int v0 = 0; v0 < full; v0 += TPB * N) {
+    typedef T vec __attribute__((ext_vector_type(VEC)));
+    float x[N][VEC], xe = -INFINITY;
+    int ie = -1;
+    {
+      vec raw[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) lp_load<T, VEC>(x[n], row, c0 + ((long)n * TPB + tid) * VEC, p.V);
-    float mt = -INFINITY;
+      for (int n = 0; n < N; ++n) {
+        const long v = min(v0 + n * TPB + tid, full - 1);          // (unconditional: the loads are in flight together)
+        if constexpr (VEC == 1) raw[n][0] = row[v];
+        else raw[n] = *(const vec*)(row + first + v * VEC);
+      }
+      if (VEC > 1 && v0 == 0) {
+        if (tid < first) ie = tid;
+        else if (tid >= VEC && first + full * VEC + tid - VEC < p.V && tid < 2 * VEC) ie = first + full * VEC + tid - VEC;
+        if (ie >= 0) xe = (float)row[ie];
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[n][j] = v0 + n * TPB + tid < full ? (float)raw[n][j] : -INFINITY;
+    }
+    float mt = xe;
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) mt = fmaxf(mt, x[n][j]);
     const float mu = mt == -INFINITY ? 0.f : mt;
-    float lt = 0.f, st = 0.f;
+    float lt, st;
+    {
+      const float d = xe - mu;
+      lt = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+      st = lt * fmaxf(d, -1e30f);
+    }
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -110,44 +162,94 @@ __global__ __launch_bounds__(TPB < 256 ? 256 : TPB) void lp_fwd_kernel(LpP p) {
       }
     lp_merge(m, l, s, mt, lt, st);
     if constexpr (TOP) {
-      unsigned taken = 0;
-      auto own = [&]() {
-        u64 k = 0;
+      float gm = mt;
+#pragma unroll
+      for (int o = GL / 2; o > 0; o >>= 1) gm = fmaxf(gm, __shfl_xor(gm, o, 64));
+      if (tid % GL == 0) q.gmax[tid / GL] = gm;
+      lp_sync<NW>();
+      // the top-th largest of the groups' maxima
+      const float own = q.gmax[lane & 15];
+      int rank = 0;
+#pragma unroll
+      for (int g = 0; g < 16; ++g) {
+        const float o = q.gmax[g];
+        rank += o > own || (o == own && g < (lane & 15));
+      }
+      const u64 at = __ballot(rank == p.top - 1);
+      const u64 last = q.list[p.top - 1];                          // 0 while fewer are known
+      float tau = __shfl(own, (int)__builtin_ctzll(at | (1ull << 63)), 64);
+      if (last) tau = fmaxf(tau, lp_value(last));
+      auto key = [&](float v, int e) { return ((u64)lp_order(v) << 32) | (0xFFFFFFFFu - (unsigned)e); };
+      auto push = [&](float v, int e) {
+        const int slot = atomicAdd(&q.count, 1);
+        if (slot < LP_CAND) q.cand[slot] = key(v, e);
+      };
+      if (mt >= tau) {
+        if (ie >= 0 && xe >= tau) push(xe, ie);
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const long e = c0 + ((long)n * TPB + tid) * VEC + j;
-            const u64 key = ((u64)lp_order(x[n][j]) << 32) | (0xFFFFFFFFu - (unsigned)e);
-            if (e >= 0 && e < p.V && !(taken >> (n * VEC + j) & 1) && key > k) k = key;
-          }
-        return k;
-      };
-      u64 mine = own(), wmax = lp_wave_max(mine);
-      if (NW > 1) {
-        __syncthreads();
-        if (lane == 0) wbest[wave] = wmax;
-        __syncthreads();
+          for (int j = 0; j < VEC; ++j)
+            if (x[n][j] >= tau && v0 + n * TPB + tid < full) push(x[n][j], first + (v0 + n * TPB + tid) * VEC + j);
       }
-      while (true) {
-        const u64 k = NW == 1 ? wmax : lp_wave_max(lane < NW ? wbest[lane] : 0);
-        const u64 last = ((u64)(unsigned)__shfl((int)(list >> 32), p.top - 1, 64) << 32) | (unsigned)__shfl((int)list, p.top - 1, 64);
-        if (k <= last) break;                          // the row is used up (0), or nothing beats the last alternative
-        const u64 prev = ((u64)(unsigned)__shfl_up((int)(list >> 32), 1, 64) << 32) | (unsigned)__shfl_up((int)list, 1, 64);
-        if (list < k) list = lane == 0 || prev > k ? k : prev;
-        // the owner drops it
-        if (NW > 1) __syncthreads();
-        if (wmax == k) {                             // (keys are unique: one wave)
-          if (mine == k) {
-            const long e = (long)(0xFFFFFFFFu - (unsigned)k) - c0;
-            const int n = (int)(e / VEC / TPB), j = (int)(e % VEC);
-            taken |= 1u << (n * VEC + j);
-            mine = own();
-          }
-          wmax = lp_wave_max(mine);
-          if (NW > 1 && lane == 0) wbest[wave] = wmax;
+      lp_sync<NW>();
+      const int count = q.count;
+      if (count <= LP_CAND) {
+        if (wave == 0) {
+          // lanes 0 - 47 hold the candidates, 48 - 63 what is in the list; keys are unique, 0 stands for nothing
+          const u64 mine = lane < count ? q.cand[lane] : lane >= 48 && lane - 48 < p.top ? q.list[lane - 48] : 0;
+          int r = 0;
+          for (int i = 0; i < count; ++i) r += q.cand[i] > mine;
+          for (int i = 0; i < p.top; ++i) r += q.list[i] > mine;
+          lp_sync<1>();
+          if (mine && r < p.top) q.list[r] = mine;
+          if (lane == 0) q.count = 0;
         }
-        if (NW > 1) __syncthreads();
+        lp_sync<NW>();
+      } else {
+        if (tid == 0) q.count = 0;
+        unsigned taken = 0;                                        // of this thread's vectors; the single element: out
+        bool out = ie < 0;
+        auto best = [&]() {                                        // largest value first, then its lowest index: no 64-bit key per element
+          float v = out ? -INFINITY : xe;
+          int e = out ? INT_MAX : ie;
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v = (taken >> (n * VEC + j)) & 1 ? v : fmaxf(v, x[n][j]);
+          if (!out && xe != v) e = INT_MAX;
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+              if (x[n][j] == v && !((taken >> (n * VEC + j)) & 1) && v0 + n * TPB + tid < full) e = min(e, first + (v0 + n * TPB + tid) * VEC + j);
+          return e == INT_MAX ? 0 : key(v, e);
+        };
+        u64 mine = best(), wmax = lp_wave_max(mine);
+        while (true) {
+          lp_sync<NW>();
+          if (lane == 0) q.wbest[wave] = wmax;
+          lp_sync<NW>();
+          const u64 k = lp_wave_max(lane < NW ? q.wbest[lane] : 0);
+          if (k <= q.list[p.top - 1]) break;                       // (uniform) used up, or nothing beats the last one
+          const u64 cur = q.list[lane & 15], prev = (lane & 15) ? q.list[(lane & 15) - 1] : ~0ull;
+          lp_sync<NW>();
+          if (wave == 0 && lane < p.top && cur < k) q.list[lane] = prev > k ? k : prev;
+          if (wmax == k) {
+            if (mine == k) {
+              const int e = (int)(0xFFFFFFFFu - (unsigned)k);
+              if (e == ie) {
+                out = true;
+              } else {
+                const int i = (e - first) - v0 * VEC;
+                taken |= 1u << ((i / VEC / TPB) * VEC + i % VEC);
+              }
+              mine = best();
+            }
+            wmax = lp_wave_max(mine);
+          }
+        }
+        lp_sync<NW>();
       }
     }
   }
@@ -176,8 +278,9 @@ __global__ __launch_bounds__(TPB < 256 ? 256 : TPB) void lp_fwd_kernel(LpP p) {
     p.stat[3 * row_i + 2] = H;
   }
   if (TOP && wave == 0 && lane < p.top) {
-    p.top_idx[row_i * p.top + lane] = (long)(0xFFFFFFFFu - (unsigned)list);
-    p.top_logp[row_i * p.top + lane] = dead ? -INFINITY : (lp_value(list) - m) - logl;
+    const u64 k = q.list[lane];
+    p.top_idx[row_i * p.top + lane] = (long)(0xFFFFFFFFu - (unsigned)k);
+    p.top_logp[row_i * p.top + lane] = dead ? -INFINITY : (lp_value(k) - m) - logl;
   }
 }
 
@@ -228,10 +331,12 @@ __global__ __launch_bounds__(256) void lp_bwd_kernel(LpP p) {
 template <typename T, bool TOP> int lp_fwd_launch(const LpP& p, hipStream_t st) {
   constexpr int CE = 16 / (int)sizeof(T);
   // a wave per row while a row fits its registers; short rows element by element (their vectors would be mostly partial)
-  if (p.V <= 512) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, 1, 8, TOP>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
-  else if (p.V <= 2048 - CE) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, CE, 32 / CE, TOP>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
-  else if (p.V <= 8192 - CE) hipLaunchKernelGGL((lp_fwd_kernel<T, 256, CE, 32 / CE, TOP>), dim3(p.rows), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((lp_fwd_kernel<T, 1024, CE, 32 / CE, TOP>), dim3(p.rows), dim3(1024), 0, st, p);
+  if (p.V <= 512) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, 1, 8, TOP, 1>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
+  else if (p.V <= 2048) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, CE, 32 / CE, TOP, 1>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
+  else if (!TOP && (p.rows >= LP_MANY || p.V <= 8192))
+    hipLaunchKernelGGL((lp_fwd_kernel<T, 256, CE, 32 / CE, TOP, 1>), dim3(p.rows), dim3(256), 0, st, p);
+  else if (p.V <= 8192) hipLaunchKernelGGL((lp_fwd_kernel<T, 256, CE, 32 / CE, TOP, 1>), dim3(p.rows), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((lp_fwd_kernel<T, 1024, CE, 32 / CE, TOP, LP_WPE>), dim3(p.rows), dim3(1024), 0, st, p);
   VLNI_LAUNCH_CHECK();
   return VLNI_OK;
 }

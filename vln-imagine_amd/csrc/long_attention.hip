@@ -1,6 +1,7 @@
 // Entry points of attention over long sequences (ops.long_attention), its mask / bias preparation and the bfloat16 instances.
 // The kernels and the mathematics are in long_attention_impl.inc.
 #include <limits.h>
+#include <math.h>
 
 #include "../../include/vlni.h"
 #include "long_attention.h"
@@ -58,9 +59,10 @@ __global__ __launch_bounds__(256) void la_dtable_kernel(const float* part, float
     e1 = k.sides == 1 && d0 == 0 && d1 >= 0 ? BL - 1 : R + LA_PAD - d0;
   }
   double a = 0.0;
-  for (int q = threadIdx.x >> 5; q < nparts; q += 8) {
-    const float* row = part + ((long)h * nparts + q) * BL;
-    for (int e = e0 + (threadIdx.x & 31); e <= e1; e += 32) a += (double)row[e];
+  for (int e = e0 + (threadIdx.x & 31); e <= e1; e += 32) {
+    const float* col = part + (long)h * nparts * BL + e;
+#pragma unroll 8
+    for (int q = threadIdx.x >> 5; q < nparts; q += 8) a += (double)col[(long)q * BL];
   }
   __shared__ double s[256];
   s[threadIdx.x] = a;
@@ -101,16 +103,21 @@ int la_fill(const VlniLongAttnArgs* a, LaP& p, LaBuckets& k) {
   return VLNI_OK;
 }
 
-// Splits of a launch along its loop: the chip works through `tiles` tiles in all at `us` microseconds a tile and CU, but no faster than the longest block
-// (`chain` tiles), whose end it partly waits for; splits shorten that and cost their partial results (float32, written and read at 4 TB/s) and a launch.
-// Measured: dK / dV of a causal 4 k pass with four key heads, 256 blocks: 301 us whole, 190 us in four.
-int la_split(double tiles, double chain, double us, double floats) {
+// Splits of a launch along its loop, by what they cost and save. `blocks` blocks walk up to `chain` tiles each, a CU takes `us` microseconds a tile.
+// Without a causal border all are alike and run in rounds of one block a CU - two where a few rows leave the loads of K and V as the bound
+// (latency: a second block's loads fly under the first one's); with one, the chip works through half of them on average (`part`) but waits for the end of
+// the longest. Splits cost their partial results (float32, written under the launch, read back at 4 TB/s) and a launch.
+// Measured: dK / dV of a causal 4 k pass with four key heads, 256 blocks: 301 us whole, 178 us in four; a token's forward pass over 8 k keys, 64 blocks of
+// heads of 128: 8 splits 55 us, 25 splits 71 us.
+int la_split(double blocks, double chain, double part, bool few, double us, double floats) {
   int best = 1;
   double least = 1e300;
+  const double slots = few ? 512.0 : 256.0;
   for (int n = 1; n <= 32 && (n == 1 || chain / n >= 2.0); ++n) {
-    const double all = tiles / 256.0, one = chain / n;
-    const double t = us * (one > all + 0.5 * one ? one : all + 0.5 * one) + (n > 1 ? 6.0 + n * floats * 8.0 / 4e6 : 0.0);
-    if (t < 0.98 * least) { best = n; least = t; }
+    const double one = ceil(chain / n), all = blocks * n * one * part / 256.0;
+    const double t = us * (part < 1.0 ? (one > all + 0.3 * one ? one : all + 0.3 * one) : slots / 256.0 * ceil(blocks * n / slots) * one) +
+                     (n > 1 ? 6.0 + n * floats * 5.0 / 4e6 : 0.0);
+    if (t < 0.97 * least) { best = n; least = t; }
   }
   return best;
 }
@@ -119,17 +126,16 @@ int la_kt_of(const VlniLongAttnArgs* a) { return a->dtype == VLNI_F32 && a->D > 
 double la_tile_us(const VlniLongAttnArgs* a, double us) {
   return us * ((a->D + 31) / 32 * 32) / 64.0 * la_kt_of(a) / 64.0 * (a->dtype == VLNI_F32 ? 7.0 : 1.0);
 }
+double la_part(const LaP& p) { return p.causal && p.PG == 1 && p.Sq > 64 ? (p.Sk - 0.5 * (p.Sq < p.Sk ? p.Sq : p.Sk)) / p.Sk : 1.0; }
 void la_grid_rows(const VlniLongAttnArgs* a, LaP& p) {
   p.nblk = cdiv((long)p.Sq * p.PG, 128);
-  const double chain = cdiv(p.Sk, la_kt_of(a)), blocks = (double)p.nblk * p.B * (p.nh / p.PG);
-  const double part = p.causal && p.PG == 1 ? (p.Sk - 0.5 * (p.Sq < p.Sk ? p.Sq : p.Sk)) / p.Sk : 1.0;
-  p.nsplit = la_split(blocks * chain * part, chain, la_tile_us(a, 0.9), (double)p.B * p.Sq * p.nh * p.D);
+  p.nsplit = la_split((double)p.nblk * p.B * (p.nh / p.PG), cdiv(p.Sk, la_kt_of(a)), la_part(p), p.Sq * p.PG <= 32, la_tile_us(a, 0.9),
+                      (double)p.B * p.Sq * p.nh * p.D);
 }
 void la_grid_keys(const VlniLongAttnArgs* a, LaP& p) {
   p.nblk = cdiv(p.Sk, 128);
-  const double chain = (double)cdiv((long)p.Sq * p.PG, la_kt_of(a)) * (p.nh / p.nkv / p.PG), blocks = (double)p.nblk * p.B * p.nkv;
-  const double part = p.causal && p.PG == 1 ? (p.Sk - 0.5 * (p.Sq < p.Sk ? p.Sq : p.Sk)) / p.Sk : 1.0;
-  p.nsplit = la_split(blocks * chain * part, chain, la_tile_us(a, 1.6), 2.0 * p.B * p.Sk * p.nkv * p.D);
+  p.nsplit = la_split((double)p.nblk * p.B * p.nkv, (double)cdiv((long)p.Sq * p.PG, la_kt_of(a)) * (p.nh / p.nkv / p.PG), la_part(p), false, la_tile_us(a, 1.6),
+                      2.0 * p.B * p.Sk * p.nkv * p.D);
 }
 long la_prep_floats(const VlniLongAttnArgs* a, const LaP& p) {
   return (a->kmask ? (long)p.B * p.SkP + (long)p.B * (p.SkP >> 6) : 0) + (a->rel_table ? (long)p.nh * p.BL : 0);
