@@ -45,8 +45,8 @@ __global__ __launch_bounds__(64) void la_prep_kernel(const float* kmask, const f
   }
 }
 
-// dtable[bucket][head] = sum of dS over the bucket's distances and all partial rows of the head; block = one (bucket, head), 8 rows x 32 distances at a
-// time, in a fixed order and in 64 bits
+// dtable[bucket][head] = sum of dS over the bucket's distances and all partial rows of the head; block = one (bucket, head), in a
+// fixed order and in 64 bits
 __global__ __launch_bounds__(256) void la_dtable_kernel(const float* part, float* dtable, LaBuckets k, int nh, int R, int BL, int nparts) {
   const int b = blockIdx.x, h = blockIdx.y, side = b / k.n, bb = b % k.n;
   const int d0 = k.first[bb], d1 = bb + 1 < k.n ? k.first[bb + 1] - 1 : INT_MAX;       // distances d0 .. d1 (none: d1 < d0)
@@ -59,10 +59,11 @@ __global__ __launch_bounds__(256) void la_dtable_kernel(const float* part, float
     e1 = k.sides == 1 && d0 == 0 && d1 >= 0 ? BL - 1 : R + LA_PAD - d0;
   }
   double a = 0.0;
-  for (int e = e0 + (threadIdx.x & 31); e <= e1; e += 32) {
+  const int lg = e1 - e0 >= 128 ? 8 : e1 - e0 >= 64 ? 7 : e1 - e0 >= 32 ? 6 : 5;       // 2^lg distances side by side
+  for (int e = e0 + (threadIdx.x & ((1 << lg) - 1)); e <= e1; e += 1 << lg) {
     const float* col = part + (long)h * nparts * BL + e;
 #pragma unroll 8
-    for (int q = threadIdx.x >> 5; q < nparts; q += 8) a += (double)col[(long)q * BL];
+    for (int q = threadIdx.x >> lg; q < nparts; q += 256 >> lg) a += (double)col[(long)q * BL];
   }
   __shared__ double s[256];
   s[threadIdx.x] = a;
