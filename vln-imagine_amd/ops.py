@@ -3567,21 +3567,55 @@ def _la_view(t):
     return t, st[:3]
 
 
-_LA_SIZES = {}
+class _LaPlan:
+    """What a call of one signature (shapes, types, options) needs besides its tensors; holds nothing of theirs."""
+    __slots__ = ("head", "first", "n_prep", "n_fwd", "n_bwd", "out_shape", "n_stat")
 
 
-def _la_sizes(head, masked, biased):
-    """(floats of prep, of the forward's work, of the backward's work) for one set of shapes."""
-    key = (*head, masked, biased)
-    n = _LA_SIZES.get(key)
-    if n is None:
+_LA_PLANS = {}
+
+
+def _la_plan(q, k, v, kmask, table, causal, scale, rel_max, bidirectional):
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"long_attention: {n} has shape {tuple(t.shape)}, expected [batch, positions, heads, head size]")
+    dt = _dt(q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"long_attention: q, k, v are {q.dtype}, {k.dtype}, {v.dtype}")
+    (B, Sq, nh, D), (_, Sk, nkv, _) = q.shape, k.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"long_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if nh < 1 or nkv < 1 or nh % nkv or nh > 1024:
+        raise ValueError(f"long_attention: {nh} heads do not share {nkv} key heads evenly (at most 1024 heads)")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"long_attention: head size {D} is not a multiple of 8 up to 128")
+    if kmask is not None and (kmask.dtype != torch.float32 or tuple(kmask.shape) != (B, Sk)):
+        raise ValueError(f"long_attention: kmask is {kmask.dtype} {tuple(kmask.shape)}, expected additive float32 {(B, Sk)}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e6:
+        raise ValueError(f"long_attention: scale {scale}")
+    p = _LaPlan()
+    sides, p.first = 0, None
+    if table is not None:
+        if table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != nh:
+            raise ValueError(f"long_attention: rel_table is {table.dtype} {tuple(table.shape)}, expected float32 [buckets, {nh}]")
+        sides = 2 if bidirectional else 1
+        n = table.shape[0] // sides
+        if table.shape[0] % sides or not 2 <= n <= 64:
+            raise ValueError(f"long_attention: {table.shape[0]} buckets on {sides} side(s): 2 to 64 a side")
+        if int(rel_max) != rel_max or not n // 2 < rel_max <= 1024:
+            raise ValueError(f"long_attention: rel_max {rel_max} with {n} buckets a side: a whole number above {n // 2}, at most 1024")
+        p.first = rel_bucket_starts(n, int(rel_max))
+    p.head = (dt, B, Sq, Sk, nh, nkv, D, int(bool(causal)), scale, 0 if p.first is None else len(p.first), sides,
+              0 if p.first is None else ctypes.addressof(p.first))
+    p.out_shape, p.n_stat = (B, Sq, nh, D), 2 * B * nh * Sq
+    p.n_prep = p.n_fwd = p.n_bwd = 0
+    if min(B, Sq, Sk) > 0:
         sizes = (ctypes.c_long * 3)()
         # (of the pointers only the presence of mask and table matters here)
-        _lib.call("vlni_long_attn_sizes", _LA_ARGS.pack(*head, *[0] * 16, int(masked), int(biased), *[0] * 10), ctypes.addressof(sizes))
-        if len(_LA_SIZES) >= 4096:
-            _LA_SIZES.clear()
-        n = _LA_SIZES[key] = tuple(sizes)
-    return n
+        _lib.call("vlni_long_attn_sizes", _LA_ARGS.pack(*p.head, *[0] * 16, int(kmask is not None), int(table is not None), *[0] * 10), ctypes.addressof(sizes))
+        p.n_prep, p.n_fwd, p.n_bwd = sizes
+    return p
 
 
 def _call_on(dev, fn, *args):
@@ -3598,49 +3632,45 @@ class _LongAttention(torch.autograd.Function):
     backward pass recomputes the probabilities. Inside an EpisodeTape it computes in every pass, the ghost pass included (on the filled buffers)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, kmask, table, causal, scale, sides, first):
+    def forward(ctx, q, k, v, kmask, table, plan):
         ctx.set_materialize_grads(False)
-        if q.numel() == 0 or k.numel() == 0:
-            ctx.head = None
+        ctx.plan = plan
+        if not plan.n_bwd:                     # nothing to attend from or to
             ctx.save_for_backward(q, k, v, table)
             return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        (B, Sq, nh, D), dev = q.shape, q.get_device()
+        dev = q.get_device()
         (q, qs), (k, ks), (v, vs) = _la_view(q), _la_view(k), _la_view(v)
         kmask = None if kmask is None else kmask.contiguous()
         table = None if table is None else table.contiguous()
-        n = 0 if first is None else len(first)
-        Sk, nkv = k.shape[1], k.shape[2]
-        head = (_dt(q), B, Sq, Sk, nh, nkv, D, causal, scale, n, sides, 0 if first is None else ctypes.addressof(first))
-        n_prep, n_fwd, n_bwd = _la_sizes(head, kmask is not None, table is not None)
-        out = q.new_empty((B, Sq, nh, D))
-        keep = torch.empty((2 * B * nh * Sq + n_prep,), dtype=torch.float32, device=q.device)          # stat, then prep
+        n_stat, n_prep, n_fwd = plan.n_stat, plan.n_prep, plan.n_fwd
+        out = q.new_empty(plan.out_shape)
+        keep = torch.empty((n_stat + n_prep,), dtype=torch.float32, device=q.device)                    # stat, then prep
         work = torch.empty((n_fwd,), dtype=torch.float32, device=q.device) if n_fwd else None
         stat = keep.data_ptr()
         mid = (*qs, *ks, *vs)
-        ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr())
-        tail = (_p(kmask), _p(table), out.data_ptr(), stat, stat + 8 * B * nh * Sq, n_prep)
-        _call_on(dev, "vlni_long_attn_fwd", _LA_ARGS.pack(*head, *ptrs, 0, *mid, 0, 0, 0, *tail, _p(work), n_fwd, 0, 0, 0, 0))
+        tail = (_p(kmask), _p(table), out.data_ptr(), stat, stat + 4 * n_stat, n_prep)
+        _call_on(dev, "vlni_long_attn_fwd", _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, *mid, 0, 0, 0, *tail, _p(work), n_fwd, 0, 0, 0, 0))
         ctx.save_for_backward(q, k, v, kmask, table, out, keep)
-        ctx.head, ctx.first, ctx.mid, ctx.tail, ctx.n_bwd = head, first, mid, tail, n_bwd
+        ctx.mid, ctx.tail = mid, tail
         return out
 
     @staticmethod
     def _backward(ctx, dout):
-        ng = ctx.needs_input_grad
+        ng, plan = ctx.needs_input_grad, ctx.plan
         if dout is None:
-            return (None,) * 9
-        if ctx.head is None:
-            return (*[torch.zeros(t.shape, dtype=t.dtype, device=t.device) if n and t is not None else None
-                      for t, n in zip(ctx.saved_tensors[:3] + (None, ctx.saved_tensors[3]), ng)], None, None, None, None)
+            return None, None, None, None, None, None
+        if not plan.n_bwd:
+            q, k, v, table = ctx.saved_tensors
+            return (*[torch.zeros(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((q, k, v, None, table), ng)], None)
         q, k, v, kmask, table, out, keep = ctx.saved_tensors
         dout, ds = _la_view(dout)
-        dq, dk, dv = q.new_empty(out.shape), q.new_empty(k.shape), q.new_empty(k.shape)
+        dq, dk, dv = q.new_empty(plan.out_shape), q.new_empty(k.shape), q.new_empty(k.shape)
         dtable = torch.empty_like(table) if ng[4] else None
-        work = torch.empty((ctx.n_bwd,), dtype=torch.float32, device=q.device)
-        args = _LA_ARGS.pack(*ctx.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *ctx.mid, *ds, *ctx.tail, work.data_ptr(), ctx.n_bwd,
+        work = torch.empty((plan.n_bwd,), dtype=torch.float32, device=q.device)
+        args = _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *ctx.mid, *ds, *ctx.tail, work.data_ptr(), plan.n_bwd,
                              dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(dtable))
         _call_on(q.get_device(), "vlni_long_attn_bwd", args)
-        return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, None, dtable, None, None, None, None
+        return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, None, dtable, None
 
     @staticmethod
     def backward(ctx, dout):
@@ -3671,40 +3701,18 @@ def long_attention(q, k, v, kmask=None, causal=False, scale=None, rel_table=None
         buckets of a side the first n // 2 hold one distance each, the others are spread over log(distance) up to rel_max (<= 1024), the last holds all
         beyond (rel_bucket_starts). rel_bidirectional: the upper half of the table is for keys behind the query; otherwise those count as distance 0.
     scale: 1 / sqrt(D) by default. Sums are float32 and in a fixed order: equal calls on one device give equal bits. No dropout, no second derivative."""
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError(f"long_attention: {n} has shape {tuple(t.shape)}, expected [batch, positions, heads, head size]")
-    _dt(q)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"long_attention: q, k, v are {q.dtype}, {k.dtype}, {v.dtype}")
-    (B, Sq, nh, D), (_, Sk, nkv, _) = q.shape, k.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
-        raise ValueError(f"long_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if nh < 1 or nkv < 1 or nh % nkv or nh > 1024:
-        raise ValueError(f"long_attention: {nh} heads do not share {nkv} key heads evenly (at most 1024 heads)")
-    if D % 8 or not 8 <= D <= 128:
-        raise ValueError(f"long_attention: head size {D} is not a multiple of 8 up to 128")
-    if kmask is not None:
-        if kmask.dtype != torch.float32 or tuple(kmask.shape) != (B, Sk):
-            raise ValueError(f"long_attention: kmask is {kmask.dtype} {tuple(kmask.shape)}, expected additive float32 {(B, Sk)}")
-        if kmask.requires_grad:
-            raise ValueError("long_attention: kmask takes no gradient")
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 1e6:
-        raise ValueError(f"long_attention: scale {scale}")
-    sides, first = 0, None
-    if rel_table is not None:
-        if rel_table.dtype != torch.float32 or rel_table.dim() != 2 or rel_table.shape[1] != nh:
-            raise ValueError(f"long_attention: rel_table is {rel_table.dtype} {tuple(rel_table.shape)}, expected float32 [buckets, {nh}]")
-        sides = 2 if rel_bidirectional else 1
-        n = rel_table.shape[0] // sides
-        if rel_table.shape[0] % sides or not 2 <= n <= 64:
-            raise ValueError(f"long_attention: {rel_table.shape[0]} buckets on {sides} side(s): 2 to 64 a side")
-        if int(rel_max) != rel_max or not n // 2 < rel_max <= 1024:
-            raise ValueError(f"long_attention: rel_max {rel_max} with {n} buckets a side: a whole number above {n // 2}, at most 1024")
-        first = rel_bucket_starts(n, int(rel_max))
+    key = (q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype, None if kmask is None else (kmask.shape, kmask.dtype),
+           None if rel_table is None else (rel_table.shape, rel_table.dtype, rel_max, rel_bidirectional), causal, scale)
+    plan = _LA_PLANS.get(key)
+    if plan is None:
+        plan = _la_plan(q, k, v, kmask, rel_table, causal, scale, rel_max, rel_bidirectional)
+        if len(_LA_PLANS) >= 4096:
+            _LA_PLANS.clear()
+        _LA_PLANS[key] = plan
+    if kmask is not None and kmask.requires_grad:
+        raise ValueError("long_attention: kmask takes no gradient")
     _same_device(q, "q", k=k, v=v, kmask=kmask, rel_table=rel_table)
-    return _LongAttention.apply(q, k, v, kmask, rel_table, int(bool(causal)), scale, sides, first)
+    return _LongAttention.apply(q, k, v, kmask, rel_table, plan)
 
 
 class _TokenLogprobs(torch.autograd.Function):
