@@ -333,9 +333,7 @@ template <typename T, bool TOP> int lp_fwd_launch(const LpP& p, hipStream_t st) 
   // a wave per row while a row fits its registers; short rows element by element (their vectors would be mostly partial)
   if (p.V <= 512) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, 1, 8, TOP, 1>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
   else if (p.V <= 2048) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, CE, 32 / CE, TOP, 1>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
-  else if (!TOP && (p.rows >= LP_MANY || p.V <= 8192))
-    hipLaunchKernelGGL((lp_fwd_kernel<T, 256, CE, 32 / CE, TOP, 1>), dim3(p.rows), dim3(256), 0, st, p);
-  else if (p.V <= 8192) hipLaunchKernelGGL((lp_fwd_kernel<T, 256, CE, 32 / CE, TOP, 1>), dim3(p.rows), dim3(256), 0, st, p);
+  else if (p.rows >= LP_MANY || p.V <= 8192) hipLaunchKernelGGL((lp_fwd_kernel<T, 256, CE, 32 / CE, TOP, TOP ? 5 : 1>), dim3(p.rows), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((lp_fwd_kernel<T, 1024, CE, 32 / CE, TOP, LP_WPE>), dim3(p.rows), dim3(1024), 0, st, p);
   VLNI_LAUNCH_CHECK();
   return VLNI_OK;
