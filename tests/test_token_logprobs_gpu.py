@@ -209,3 +209,17 @@ def test_gradient_against_differences(ops):
         lp, ent, _, _ = ops.token_logprobs(x + s * d, t)
         val.append(lp.double().sum() + 0.7 * ent.double().sum())
     assert abs(((val[0] - val[1]) / (2 * h)).item() - (lg.grad.double() * d.double()).sum().item()) < 2e-3
+
+
+@pytest.mark.parametrize("V", [37, 1500, 5000, 30000])
+def test_rows_with_nan(ops, V):
+    """NaN in a row gives NaN for that row alone; the alternatives' indices stay inside it."""
+    x, t = _rand((5, V), F32, 3), torch.arange(5).cuda()
+    want = ops.token_logprobs(x, t, top=8)
+    x[1, 20], x[3] = float("nan"), float("nan")
+    logp, ent, tl, ti = ops.token_logprobs(x, t, top=8)
+    good = torch.tensor([0, 2, 4]).cuda()
+    assert all(torch.equal(a[good], b[good]) for a, b in zip((logp, ent, tl, ti), want))
+    for r in (1, 3):
+        assert logp[r].isnan() and ent[r].isnan() and tl[r].isnan().all()
+        assert ((ti[r] >= 0) & (ti[r] < V)).all()

@@ -19,9 +19,6 @@
 namespace {
 
 constexpr int LP_MAXTOP = 16, LP_MANY = 1024;
-#ifndef LP_WPE
-#define LP_WPE 4
-#endif
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 typedef unsigned long long u64;
 
@@ -162,23 +159,27 @@ __global__ __launch_bounds__(TPB < 256 ? 256 : TPB, WPE) void lp_fwd_kernel(LpP 
       }
     lp_merge(m, l, s, mt, lt, st);
     if constexpr (TOP) {
-      float gm = mt;
+      // what may be among the `top` best of the row: nothing below the list's last, or - while the list is not full, its last then 0 - below the
+      // top-th largest of the groups' maxima
+      const u64 last = q.list[p.top - 1];
+      float tau;
+      if (last) {                                                  // (uniform)
+        tau = lp_value(last);
+      } else {
+        float gm = mt;
 #pragma unroll
-      for (int o = GL / 2; o > 0; o >>= 1) gm = fmaxf(gm, __shfl_xor(gm, o, 64));
-      if (tid % GL == 0) q.gmax[tid / GL] = gm;
-      lp_sync<NW>();
-      // the top-th largest of the groups' maxima
-      const float own = q.gmax[lane & 15];
-      int rank = 0;
+        for (int o = GL / 2; o > 0; o >>= 1) gm = fmaxf(gm, __shfl_xor(gm, o, 64));
+        if (tid % GL == 0) q.gmax[tid / GL] = gm;
+        lp_sync<NW>();
+        const float own = q.gmax[lane & 15];
+        int rank = 0;
 #pragma unroll
-      for (int g = 0; g < 16; ++g) {
-        const float o = q.gmax[g];
-        rank += o > own || (o == own && g < (lane & 15));
+        for (int g = 0; g < 16; ++g) {
+          const float o = q.gmax[g];
+          rank += o > own || (o == own && g < (lane & 15));
+        }
+        tau = __shfl(own, (int)__builtin_ctzll(__ballot(rank == p.top - 1) | (1ull << 63)), 64);
       }
-      const u64 at = __ballot(rank == p.top - 1);
-      const u64 last = q.list[p.top - 1];                          // 0 while fewer are known
-      float tau = __shfl(own, (int)__builtin_ctzll(at | (1ull << 63)), 64);
-      if (last) tau = fmaxf(tau, lp_value(last));
       auto key = [&](float v, int e) { return ((u64)lp_order(v) << 32) | (0xFFFFFFFFu - (unsigned)e); };
       auto push = [&](float v, int e) {
         const int slot = atomicAdd(&q.count, 1);
@@ -279,8 +280,8 @@ __global__ __launch_bounds__(TPB < 256 ? 256 : TPB, WPE) void lp_fwd_kernel(LpP 
   }
   if (TOP && wave == 0 && lane < p.top) {
     const u64 k = q.list[lane];
-    p.top_idx[row_i * p.top + lane] = (long)(0xFFFFFFFFu - (unsigned)k);
-    p.top_logp[row_i * p.top + lane] = dead ? -INFINITY : (lp_value(k) - m) - logl;
+    p.top_idx[row_i * p.top + lane] = k ? (long)(0xFFFFFFFFu - (unsigned)k) : lane;        // (a row of NaN has no largest elements)
+    p.top_logp[row_i * p.top + lane] = dead ? -INFINITY : (lp_value(k) - m) - logl;        // (0 is the key of a NaN)
   }
 }
 
@@ -330,11 +331,14 @@ __global__ __launch_bounds__(256) void lp_bwd_kernel(LpP p) {
 
 template <typename T, bool TOP> int lp_fwd_launch(const LpP& p, hipStream_t st) {
   constexpr int CE = 16 / (int)sizeof(T);
-  // a wave per row while a row fits its registers; short rows element by element (their vectors would be mostly partial)
+  // a wave per row while a row fits its registers; short rows element by element (their vectors would be mostly partial); long rows of a launch that
+  // fills the chip a block of 256 each, of a small one a block of 1024 (8 x 30522 float32, top 5: 12.6 us, with 256: 31). The alternatives' kernel at
+  // five waves a SIMD: what it waits for are its own barriers, and 15 registers in memory cost less than the fourth wave's place (2048 x 30522 bf16,
+  // top 8: 53 us, unrestricted 88)
   if (p.V <= 512) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, 1, 8, TOP, 1>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
   else if (p.V <= 2048) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, CE, 32 / CE, TOP, 1>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
   else if (p.rows >= LP_MANY || p.V <= 8192) hipLaunchKernelGGL((lp_fwd_kernel<T, 256, CE, 32 / CE, TOP, TOP ? 5 : 1>), dim3(p.rows), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((lp_fwd_kernel<T, 1024, CE, 32 / CE, TOP, LP_WPE>), dim3(p.rows), dim3(1024), 0, st, p);
+  else hipLaunchKernelGGL((lp_fwd_kernel<T, 1024, CE, 32 / CE, TOP, 4>), dim3(p.rows), dim3(1024), 0, st, p);
   VLNI_LAUNCH_CHECK();
   return VLNI_OK;
 }
