@@ -3647,11 +3647,9 @@ class _LongAttention(torch.autograd.Function):
         keep = torch.empty((n_stat + n_prep,), dtype=torch.float32, device=q.device)                    # stat, then prep
         work = torch.empty((n_fwd,), dtype=torch.float32, device=q.device) if n_fwd else None
         stat = keep.data_ptr()
-        mid = (*qs, *ks, *vs)
-        tail = (_p(kmask), _p(table), out.data_ptr(), stat, stat + 4 * n_stat, n_prep)
-        _call_on(dev, "vlni_long_attn_fwd", _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, *mid, 0, 0, 0, *tail, _p(work), n_fwd, 0, 0, 0, 0))
+        _call_on(dev, "vlni_long_attn_fwd", _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, *qs, *ks, *vs, 0, 0, 0, _p(kmask), _p(table),
+                                                          out.data_ptr(), stat, stat + 4 * n_stat, n_prep, _p(work), n_fwd, 0, 0, 0, 0))
         ctx.save_for_backward(q, k, v, kmask, table, out, keep)
-        ctx.mid, ctx.tail = mid, tail
         return out
 
     @staticmethod
@@ -3662,12 +3660,16 @@ class _LongAttention(torch.autograd.Function):
         if not plan.n_bwd:
             q, k, v, table = ctx.saved_tensors
             return (*[torch.zeros(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((q, k, v, None, table), ng)], None)
+        # (checkpointing and offloading hand back other tensors than were saved, in other layouts: no address or stride of the forward pass holds)
         q, k, v, kmask, table, out, keep = ctx.saved_tensors
-        dout, ds = _la_view(dout)
+        (q, qs), (k, ks), (v, vs), (dout, ds) = _la_view(q), _la_view(k), _la_view(v), _la_view(dout)
+        kmask, table = None if kmask is None else kmask.contiguous(), None if table is None else table.contiguous()
+        out, stat = out.contiguous(), keep.data_ptr()
         dq, dk, dv = q.new_empty(plan.out_shape), q.new_empty(k.shape), q.new_empty(k.shape)
         dtable = torch.empty_like(table) if ng[4] else None
         work = torch.empty((plan.n_bwd,), dtype=torch.float32, device=q.device)
-        args = _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *ctx.mid, *ds, *ctx.tail, work.data_ptr(), plan.n_bwd,
+        args = _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *qs, *ks, *vs, *ds, _p(kmask), _p(table),
+                             out.data_ptr(), stat, stat + 4 * plan.n_stat, plan.n_prep, work.data_ptr(), plan.n_bwd,
                              dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(dtable))
         _call_on(q.get_device(), "vlni_long_attn_bwd", args)
         return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, None, dtable, None
@@ -3773,7 +3775,7 @@ def token_logprobs(logits, target, top=0, ignore_index=-100):
     float32 [...], float32 [...], float32 and int64 [..., top] (None with top = 0), the alternatives in falling order, equal ones by lowest index.
     logp and entropy are differentiable (policy gradient with entropy bonus, r2r/agent_cmt.py:569-574,702-744; masked-token losses), the alternatives
     are not. A target equal to ignore_index, or outside [0, V), has logp 0 and sends no gradient through it; the latter are counted
-    (`watch_index_errors` / `index_errors`). A row of -inf only: logp -inf, entropy 0, no gradient. top <= 16."""
+    (`watch_index_errors` / `index_errors`). A row of -inf only: logp -inf, entropy 0, no gradient; one that holds NaN gives NaN. top <= 16."""
     _dt(logits)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"token_logprobs: logits {tuple(logits.shape)}")
