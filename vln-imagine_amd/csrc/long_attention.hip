@@ -104,38 +104,48 @@ int la_fill(const VlniLongAttnArgs* a, LaP& p, LaBuckets& k) {
   return VLNI_OK;
 }
 
-// Splits of a launch along its loop, by what they cost and save. `blocks` blocks walk up to `chain` tiles each, a CU takes `us` microseconds a tile.
-// Without a causal border all are alike and run in rounds of one block a CU - two where a few rows leave the loads of K and V as the bound
-// (latency: a second block's loads fly under the first one's); with one, the chip works through half of them on average (`part`) but waits for the end of
-// the longest. Splits cost their partial results (float32, written under the launch, read back at 4 TB/s) and a launch.
-// Measured: dK / dV of a causal 4 k pass with four key heads, 256 blocks: 301 us whole, 178 us in four; a token's forward pass over 8 k keys, 64 blocks of
-// heads of 128: 8 splits 55 us, 25 splits 71 us.
-int la_split(double blocks, double chain, double part, bool few, double us, double floats) {
+// Splits of a launch along its loop, by what they cost and save. `blocks` blocks walk up to `chain` tiles each; a tile costs a CU `us` microseconds where
+// other blocks fill its waits, and `alone` pass before a block begins its next one.
+// Without a causal border all blocks are alike and run in rounds of one block a CU - two where a few rows leave the loads of K and V as the bound
+// (latency: a second block's loads fly under the first one's). With one, the chip works through half of the tiles on average (`part`) but waits for the
+// end of the longest chain. Splits cost a launch and their partial results, float32, written and read again at 4.5 TB/s.
+// Measured (heads of 64, whole -> split, with what joins them): dK / dV of a causal 4 k pass with four key heads, 256 blocks: 406 us -> in four 141 + 13;
+// 3 x 1501 causal positions of 8 heads with a bias, 288 blocks, forward: 42 -> in three 27 + 9; 1024 positions of 12 heads, 96 blocks, forward: 25 -> in
+// four 15 + 5; 2 x 512: 14 -> in two 12 + 5, so not split. A token over 8 k keys, 64 blocks of heads of 128: in eight 45 + 5, in 25 71.
+int la_split(double blocks, double chain, double part, bool few, const double (&tile)[2], double floats) {
   int best = 1;
   double least = 1e300;
-  const double slots = few ? 512.0 : 256.0;
+  const double us = tile[0], alone = tile[1], slots = few ? 512.0 : 256.0;
   for (int n = 1; n <= 32 && (n == 1 || chain / n >= 2.0); ++n) {
-    const double one = ceil(chain / n), all = blocks * n * one * part / 256.0;
-    const double t = us * (part < 1.0 ? (one > all + 0.3 * one ? one : all + 0.3 * one) : slots / 256.0 * ceil(blocks * n / slots) * one) +
-                     (n > 1 ? 6.0 + n * floats * 5.0 / 4e6 : 0.0);
-    if (t < 0.97 * least) { best = n; least = t; }
+    const double one = ceil(chain / n), all = us * (part < 1.0 ? blocks * n * one * part / 256.0 + 0.3 * one : slots / 256.0 * ceil(blocks * n / slots) * one);
+    const double t = (!few && alone * one > all ? alone * one : all) + (n > 1 ? 5.0 + n * floats * 8.0 / 4.5e6 : 0.0);
+    if (t < 0.98 * least) { best = n; least = t; }
   }
   return best;
 }
 int la_kt_of(const VlniLongAttnArgs* a) { return a->dtype == VLNI_F32 && a->D > 64 ? 32 : 64; }
-// microseconds of a 64 x 128 tile on a CU: measured at D = 64, 16 bit; float32 products run at a tenth of the rate
-double la_tile_us(const VlniLongAttnArgs* a, double us) {
-  return us * ((a->D + 31) / 32 * 32) / 64.0 * la_kt_of(a) / 64.0 * (a->dtype == VLNI_F32 ? 7.0 : 1.0);
+// `us` and `alone` of a tile, for rows (forward, dQ) or keys (dK / dV): measured at D = 64 and, in 16 bits, half of it with a head's size; float32's
+// products leave other blocks nothing to fill
+void la_tile(const VlniLongAttnArgs* a, bool keys, double (&tile)[2]) {
+  const int dp = (a->D + 31) / 32 * 32;
+  if (a->dtype == VLNI_F32) tile[0] = tile[1] = (keys ? 12.5 : 6.0) * dp / 64 * la_kt_of(a) / 64;
+  else {
+    tile[0] = (keys ? 1.2 : 0.72) * (64 + dp) / 128;
+    tile[1] = (keys ? 2.4 : 1.7) * (64 + dp) / 128;
+  }
 }
 double la_part(const LaP& p) { return p.causal && p.PG == 1 && p.Sq > 64 ? (p.Sk - 0.5 * (p.Sq < p.Sk ? p.Sq : p.Sk)) / p.Sk : 1.0; }
 void la_grid_rows(const VlniLongAttnArgs* a, LaP& p) {
+  double tile[2];
+  la_tile(a, false, tile);
   p.nblk = cdiv((long)p.Sq * p.PG, 128);
-  p.nsplit = la_split((double)p.nblk * p.B * (p.nh / p.PG), cdiv(p.Sk, la_kt_of(a)), la_part(p), p.Sq * p.PG <= 32, la_tile_us(a, 0.9),
-                      (double)p.B * p.Sq * p.nh * p.D);
+  p.nsplit = la_split((double)p.nblk * p.B * (p.nh / p.PG), cdiv(p.Sk, la_kt_of(a)), la_part(p), p.Sq * p.PG <= 32, tile, (double)p.B * p.Sq * p.nh * p.D);
 }
 void la_grid_keys(const VlniLongAttnArgs* a, LaP& p) {
+  double tile[2];
+  la_tile(a, true, tile);
   p.nblk = cdiv(p.Sk, 128);
-  p.nsplit = la_split((double)p.nblk * p.B * p.nkv, (double)cdiv((long)p.Sq * p.PG, la_kt_of(a)) * (p.nh / p.nkv / p.PG), la_part(p), false, la_tile_us(a, 1.6),
+  p.nsplit = la_split((double)p.nblk * p.B * p.nkv, (double)cdiv((long)p.Sq * p.PG, la_kt_of(a)) * (p.nh / p.nkv / p.PG), la_part(p), false, tile,
                       2.0 * p.B * p.Sk * p.nkv * p.D);
 }
 long la_prep_floats(const VlniLongAttnArgs* a, const LaP& p) {
