@@ -4,7 +4,7 @@ Bounds are elementwise and follow from the arithmetic, with u = eps / 2 of the 1
   scores   |dt| <= 2^-24 (D scale <|q|,|k|> + 4 |t| + 4 |row maximum|), so P is off by at most epsP = 2 max|dt| + 2^-20 relative (the float32 exp2 and the sum's own
            rounding are inside 2^-20), sums of n terms by n 2^-24 of the sum of magnitudes;
   out      (u + epsP + n 2^-24) P|V| + u |out|            (P rounded once, out rounded once)
-  delta    |dO| . (error of out) + D 2^-24 |dO|.|out|
+  delta    |dO| . (error of out, whose own rounding is kept beside it to u^2 |out| in 16 bits) + D 2^-24 |dO|.|out|
   dS       u |dS| + epsP |dS| + P (error of delta + D 2^-24 |dO|.|V|)
   dV, dQ, dK   the same sums over the errors of P and dS, and one rounding of the result; the table's gradient sums dS before it is rounded
            and with delta from the rows' own sums.
@@ -79,7 +79,8 @@ def _reference(q, k, v, dout, kmask, causal, scale, table, rel_max, bidir):
     res = {"out": (out, eO)}
     dP = dO @ V.transpose(2, 3)
     delta = (dO * out).sum(-1, keepdim=True)
-    edelta = (dO.abs() * (eO + D * e24 * out.abs())).sum(-1, keepdim=True)
+    eD = eO if dt == F32 else eO - (u - u * u) * out.abs()
+    edelta = (dO.abs() * (eD + D * e24 * out.abs())).sum(-1, keepdim=True)
     dS = P * (dP - delta)
     eS = epsP * dS.abs() + P * (edelta + D * e24 * (dO.abs() @ V.abs().transpose(2, 3)) + 4 * e24 * (dP.abs() + delta.abs()))
     aS = dS.abs()

@@ -13,18 +13,18 @@ class Args(ctypes.Structure):                # VlniLongAttnArgs (include/vlni.h)
                [("scale", ctypes.c_float), ("rel_n", ctypes.c_int), ("rel_sides", ctypes.c_int), ("rel_first", ctypes.c_void_p)] + \
                [(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout")] + \
                [(n, ctypes.c_long * 3) for n in ("q_stride", "k_stride", "v_stride", "do_stride")] + \
-               [(n, ctypes.c_void_p) for n in ("kmask", "rel_table", "out", "stat")] + \
+               [(n, ctypes.c_void_p) for n in ("kmask", "rel_table", "out", "out_low", "stat")] + \
                [("prep", ctypes.c_void_p), ("prep_floats", ctypes.c_long), ("work", ctypes.c_void_p), ("work_floats", ctypes.c_long)] + \
                [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "dtable")]
 
 
 def test_packed_arguments_have_the_structures_layout():
     assert ops._LA_ARGS.size == ctypes.sizeof(Args)
-    vals = list(range(1, 9)) + [0.5] + list(range(10, 41))
+    vals = list(range(1, 9)) + [0.5] + list(range(10, 42))
     a = Args.from_buffer_copy(ops._LA_ARGS.pack(*vals))
     assert (a.dtype, a.causal, a.scale, a.rel_sides, a.rel_first, a.q, a.dout) == (1, 8, 0.5, 11, 12, 13, 16)
     assert list(a.q_stride) == [17, 18, 19] and list(a.do_stride) == [26, 27, 28]
-    assert (a.kmask, a.rel_table, a.out, a.stat, a.prep, a.prep_floats, a.work, a.work_floats, a.dq, a.dtable) == (29, 30, 31, 32, 33, 34, 35, 36, 37, 40)
+    assert (a.kmask, a.rel_table, a.out, a.out_low, a.stat, a.prep, a.prep_floats, a.work, a.work_floats, a.dq, a.dtable) == (29, 30, 31, 32, 33, 34, 35, 36, 37, 38, 41)
 
 
 def _qkv(B=2, Sq=5, Sk=7, nh=4, nkv=2, D=64, dtype=torch.float32):
@@ -82,7 +82,7 @@ def test_c_entry_points_refuse():
     three = (ctypes.c_long * 3)
     first = (ctypes.c_int * 4)(0, 1, 2, 4)
     wrong = [dict(dtype=3), dict(B=0), dict(Sq=0), dict(Sk=-1), dict(nkv=3), dict(D=60), dict(D=192), dict(scale=0.0), dict(Sk=(1 << 24) + 1), dict(q=4104), dict(k=0), dict(v=4100),
-             dict(k_stride=three(1, 64, 64)), dict(out=0), dict(stat=0), dict(kmask=4096), dict(prep=4096, prep_floats=3, kmask=4096),
+             dict(k_stride=three(1, 64, 64)), dict(out=0), dict(out_low=4104), dict(stat=0), dict(kmask=4096), dict(prep=4096, prep_floats=3, kmask=4096),
              dict(rel_table=4096, rel_n=4, rel_sides=2), dict(rel_table=4096, rel_n=65, rel_sides=1, rel_first=ctypes.addressof(first)),
              dict(rel_table=4096, rel_n=3, rel_sides=3, rel_first=ctypes.addressof(first))]
     for kw in wrong:

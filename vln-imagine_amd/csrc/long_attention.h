@@ -11,7 +11,7 @@ constexpr int LA_MAXB = 64;                  // buckets per side
 struct LaP {
   const void *q, *k, *v, *dout;
   long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, d_b, d_s, d_h;      // strides in elements
-  void* out;                   // [B, Sq, nh, D]
+  void *out, *low;             // [B, Sq, nh, D] each: the result, and what its rounding to 16 bits took (null: nobody wants it)
   float* lse; float* rl;       // [B, nh, Sq] each: see the masks' comment above
   float* delta;                // [B, nh, Sq]
   const float* kml;            // [B, SkP] mask in units of log2, -inf behind Sk; null without a mask

@@ -216,7 +216,8 @@ extern "C" int vlni_long_attn_fwd(const VlniLongAttnArgs* a, void* stream) {
   LA_TRY(la_operand("q", a->q, a->q_stride, a->dtype));
   LA_TRY(la_operand("k", a->k, a->k_stride, a->dtype));
   LA_TRY(la_operand("v", a->v, a->v_stride, a->dtype));
-  VLNI_CHECK(a->out && a->stat && (uintptr_t)a->out % 16 == 0, VLNI_EINVAL, "long_attn: out %p, stat %p", a->out, (void*)a->stat);
+  VLNI_CHECK(a->out && a->stat && ((uintptr_t)a->out | (uintptr_t)a->out_low) % 16 == 0, VLNI_EINVAL, "long_attn: out %p, out_low %p, stat %p", a->out,
+             a->out_low, (void*)a->stat);
   const long n = (long)p.B * p.Sq * p.nh;
   const long need = la_prep_floats(a, p), work = la_fwd_work(a, p);
   VLNI_CHECK(!need || (a->prep && a->prep_floats >= need), VLNI_EINVAL, "long_attn: prep holds %ld floats, %ld are needed", a->prep ? a->prep_floats : 0, need);
@@ -235,7 +236,7 @@ extern "C" int vlni_long_attn_fwd(const VlniLongAttnArgs* a, void* stream) {
   p.q_b = a->q_stride[0]; p.q_s = a->q_stride[1]; p.q_h = a->q_stride[2];
   p.k_b = a->k_stride[0]; p.k_s = a->k_stride[1]; p.k_h = a->k_stride[2];
   p.v_b = a->v_stride[0]; p.v_s = a->v_stride[1]; p.v_h = a->v_stride[2];
-  p.out = a->out; p.lse = a->stat; p.rl = a->stat + n;
+  p.out = a->out; p.low = a->dtype == VLNI_F32 ? nullptr : a->out_low; p.lse = a->stat; p.rl = a->stat + n;
   la_grid_rows(a, p);
   p.part = (float*)a->work;
   p.part_ml = p.part + (long)p.nsplit * n * p.D;
@@ -249,7 +250,8 @@ extern "C" int vlni_long_attn_bwd(const VlniLongAttnArgs* a, void* stream) {
   LA_TRY(la_operand("k", a->k, a->k_stride, a->dtype));
   LA_TRY(la_operand("v", a->v, a->v_stride, a->dtype));
   LA_TRY(la_operand("dout", a->dout, a->do_stride, a->dtype));
-  VLNI_CHECK(a->out && a->stat && (uintptr_t)a->out % 16 == 0, VLNI_EINVAL, "long_attn: out %p, stat %p", a->out, (void*)a->stat);
+  VLNI_CHECK(a->out && a->stat && ((uintptr_t)a->out | (uintptr_t)a->out_low) % 16 == 0, VLNI_EINVAL, "long_attn: out %p, out_low %p, stat %p", a->out,
+             a->out_low, (void*)a->stat);
   VLNI_CHECK(a->dq && a->dk && a->dv && ((uintptr_t)a->dq | (uintptr_t)a->dk | (uintptr_t)a->dv) % 16 == 0, VLNI_EINVAL, "long_attn: dq %p, dk %p, dv %p",
              a->dq, a->dk, a->dv);
   VLNI_CHECK(!a->dtable || a->rel_table, VLNI_EINVAL, "long_attn: a table gradient without a table");
@@ -266,7 +268,7 @@ extern "C" int vlni_long_attn_bwd(const VlniLongAttnArgs* a, void* stream) {
   p.k_b = a->k_stride[0]; p.k_s = a->k_stride[1]; p.k_h = a->k_stride[2];
   p.v_b = a->v_stride[0]; p.v_s = a->v_stride[1]; p.v_h = a->v_stride[2];
   p.d_b = a->do_stride[0]; p.d_s = a->do_stride[1]; p.d_h = a->do_stride[2];
-  p.out = a->out; p.lse = a->stat; p.rl = a->stat + n;
+  p.out = a->out; p.low = a->dtype == VLNI_F32 ? nullptr : a->out_low; p.lse = a->stat; p.rl = a->stat + n;
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   float* f = (float*)a->work;
   p.delta = f;

@@ -3531,7 +3531,7 @@ def cosine(x, y):
 #  attention over long sequences, token log probabilities
 # =====================================================================================
 # VlniLongAttnArgs (include/vlni.h), packed in one go: filling a ctypes structure field by field costs more than launching a kernel
-_LA_ARGS = struct.Struct("@8ifiiP4P12l4PPlPl4P")
+_LA_ARGS = struct.Struct("@8ifiiP4P12l5PPlPl4P")
 
 
 _REL_FIRST = {}
@@ -3613,7 +3613,7 @@ def _la_plan(q, k, v, kmask, table, causal, scale, rel_max, bidirectional):
     if min(B, Sq, Sk) > 0:
         sizes = (ctypes.c_long * 3)()
         # (of the pointers only the presence of mask and table matters here)
-        _lib.call("vlni_long_attn_sizes", _LA_ARGS.pack(*p.head, *[0] * 16, int(kmask is not None), int(table is not None), *[0] * 10), ctypes.addressof(sizes))
+        _lib.call("vlni_long_attn_sizes", _LA_ARGS.pack(*p.head, *[0] * 16, int(kmask is not None), int(table is not None), *[0] * 11), ctypes.addressof(sizes))
         p.n_prep, p.n_fwd, p.n_bwd = sizes
     return p
 
@@ -3628,11 +3628,11 @@ def _call_on(dev, fn, *args):
 
 
 class _LongAttention(torch.autograd.Function):
-    """softmax(scale q k^T + kmask + bias by distance) v without the score matrix (vlni_long_attn_*). Saves q, k, v, out and two floats per row; the
-    backward pass recomputes the probabilities. Inside an EpisodeTape it computes in every pass, the ghost pass included (on the filled buffers)."""
+    """softmax(scale q k^T + kmask + bias by distance) v without the score matrix (vlni_long_attn_*). Saves q, k, v, out (in 16 bits: with what its
+    rounding took) and two floats per row; the backward pass recomputes the probabilities. Inside an EpisodeTape it computes in every pass, the ghost pass included (on the filled buffers)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, kmask, table, plan):
+    def forward(ctx, q, k, v, kmask, table, plan, train):
         ctx.set_materialize_grads(False)
         ctx.plan = plan
         if not plan.n_bwd:                     # nothing to attend from or to
@@ -3644,35 +3644,36 @@ class _LongAttention(torch.autograd.Function):
         table = None if table is None else table.contiguous()
         n_stat, n_prep, n_fwd = plan.n_stat, plan.n_prep, plan.n_fwd
         out = q.new_empty(plan.out_shape)
+        low = q.new_empty(plan.out_shape) if train and q.dtype is not torch.float32 else None
         keep = torch.empty((n_stat + n_prep,), dtype=torch.float32, device=q.device)                    # stat, then prep
         work = torch.empty((n_fwd,), dtype=torch.float32, device=q.device) if n_fwd else None
         stat = keep.data_ptr()
         _call_on(dev, "vlni_long_attn_fwd", _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, *qs, *ks, *vs, 0, 0, 0, _p(kmask), _p(table),
-                                                          out.data_ptr(), stat, stat + 4 * n_stat, n_prep, _p(work), n_fwd, 0, 0, 0, 0))
-        ctx.save_for_backward(q, k, v, kmask, table, out, keep)
+                                                          out.data_ptr(), _p(low), stat, stat + 4 * n_stat, n_prep, _p(work), n_fwd, 0, 0, 0, 0))
+        ctx.save_for_backward(q, k, v, kmask, table, out, low, keep)
         return out
 
     @staticmethod
     def _backward(ctx, dout):
         ng, plan = ctx.needs_input_grad, ctx.plan
         if dout is None:
-            return None, None, None, None, None, None
+            return None, None, None, None, None, None, None
         if not plan.n_bwd:
             q, k, v, table = ctx.saved_tensors
-            return (*[torch.zeros(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((q, k, v, None, table), ng)], None)
+            return (*[torch.zeros(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((q, k, v, None, table), ng)], None, None)
         # (checkpointing and offloading hand back other tensors than were saved, in other layouts: no address or stride of the forward pass holds)
-        q, k, v, kmask, table, out, keep = ctx.saved_tensors
+        q, k, v, kmask, table, out, low, keep = ctx.saved_tensors
         (q, qs), (k, ks), (v, vs), (dout, ds) = _la_view(q), _la_view(k), _la_view(v), _la_view(dout)
         kmask, table = None if kmask is None else kmask.contiguous(), None if table is None else table.contiguous()
-        out, stat = out.contiguous(), keep.data_ptr()
+        out, low, stat = out.contiguous(), None if low is None else low.contiguous(), keep.data_ptr()
         dq, dk, dv = q.new_empty(plan.out_shape), q.new_empty(k.shape), q.new_empty(k.shape)
         dtable = torch.empty_like(table) if ng[4] else None
         work = torch.empty((plan.n_bwd,), dtype=torch.float32, device=q.device)
         args = _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *qs, *ks, *vs, *ds, _p(kmask), _p(table),
-                             out.data_ptr(), stat, stat + 4 * plan.n_stat, plan.n_prep, work.data_ptr(), plan.n_bwd,
+                             out.data_ptr(), _p(low), stat, stat + 4 * plan.n_stat, plan.n_prep, work.data_ptr(), plan.n_bwd,
                              dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(dtable))
         _call_on(q.get_device(), "vlni_long_attn_bwd", args)
-        return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, None, dtable, None
+        return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, None, dtable, None, None
 
     @staticmethod
     def backward(ctx, dout):
@@ -3714,7 +3715,8 @@ def long_attention(q, k, v, kmask=None, causal=False, scale=None, rel_table=None
     if kmask is not None and kmask.requires_grad:
         raise ValueError("long_attention: kmask takes no gradient")
     _same_device(q, "q", k=k, v=v, kmask=kmask, rel_table=rel_table)
-    return _LongAttention.apply(q, k, v, kmask, rel_table, plan)
+    train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (rel_table is not None and rel_table.requires_grad))
+    return _LongAttention.apply(q, k, v, kmask, rel_table, plan, train)
 
 
 class _TokenLogprobs(torch.autograd.Function):
