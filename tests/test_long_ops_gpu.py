@@ -157,3 +157,12 @@ def test_checkpointed_and_offloaded_tensors(ops):
         with torch.autograd.graph.save_on_cpu():                   # comes back contiguous: in other strides than it was saved in
             return f(*a)
     assert all(torch.equal(a, b) for a, b in zip(plain, _both(ops, offloaded)))
+
+
+def test_a_scale_on_the_device_counts_with_its_value_of_the_call(ops):
+    q = torch.randn((1, 40, 2, 64), generator=torch.Generator().manual_seed(1)).cuda()
+    scale = torch.tensor(0.125, device="cuda")
+    a = ops.long_attention(q, q, q, scale=scale)
+    scale.fill_(0.5)
+    b = ops.long_attention(q, q, q, scale=scale)
+    assert torch.equal(a, ops.long_attention(q, q, q, scale=0.125)) and torch.equal(b, ops.long_attention(q, q, q, scale=0.5)) and not torch.equal(a, b)

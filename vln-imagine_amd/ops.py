@@ -3704,6 +3704,9 @@ def long_attention(q, k, v, kmask=None, causal=False, scale=None, rel_table=None
         buckets of a side the first n // 2 hold one distance each, the others are spread over log(distance) up to rel_max (<= 1024), the last holds all
         beyond (rel_bucket_starts). rel_bidirectional: the upper half of the table is for keys behind the query; otherwise those count as distance 0.
     scale: 1 / sqrt(D) by default. Sums are float32 and in a fixed order: equal calls on one device give equal bits. No dropout, no second derivative."""
+    # (plain values, so that a plan is never found again by the identity of an argument whose value has changed)
+    causal, rel_bidirectional = bool(causal), bool(rel_bidirectional)
+    scale, rel_max = None if scale is None else float(scale), float(rel_max)
     key = (q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype, None if kmask is None else (kmask.shape, kmask.dtype),
            None if rel_table is None else (rel_table.shape, rel_table.dtype, rel_max, rel_bidirectional), causal, scale)
     plan = _LA_PLANS.get(key)
