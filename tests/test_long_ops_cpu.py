@@ -57,7 +57,9 @@ def test_token_logprobs_refuses():
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.token_logprobs(x, t)
     for args, kw in (((x, t.int()), {}), ((x, t[:2]), {}), ((x, t[:, None]), {}), ((x, t), dict(top=11)), ((torch.zeros(3, 40), t), dict(top=17)), ((x, t), dict(top=-1)),
-                     ((torch.zeros(3, 0), t), {})):
+                     ((torch.zeros(3, 0), t), {}),
+                     ((torch.empty(2, (1 << 28) + 1, device="meta"), torch.empty(2, dtype=torch.int64, device="meta")), {}),
+                     ((torch.empty(1 << 31, 1, device="meta"), torch.empty(1 << 31, dtype=torch.int64, device="meta")), {})):
         with pytest.raises(ValueError):
             ops.token_logprobs(*args, **kw)
     with pytest.raises(TypeError):

@@ -3788,7 +3788,7 @@ def token_logprobs(logits, target, top=0, ignore_index=-100):
         raise ValueError(f"token_logprobs: target is {target.dtype} {tuple(target.shape)}, expected int64 {tuple(logits.shape[:-1])}")
     if not 0 <= top <= min(16, logits.shape[-1]):
         raise ValueError(f"token_logprobs: top = {top} of {logits.shape[-1]} (at most 16)")
-    if logits.shape[-1] >= 1 << 30:
-        raise ValueError(f"token_logprobs: {logits.shape[-1]} columns")
+    if logits.shape[-1] > 1 << 28 or target.numel() >= 1 << 31:
+        raise ValueError(f"token_logprobs: logits {tuple(logits.shape)}: at most 2^28 columns and 2^31 - 1 rows")
     _same_device(logits, "logits", target=target)
     return _TokenLogprobs.apply(logits, target, int(top), int(ignore_index))
