@@ -166,3 +166,50 @@ def test_a_scale_on_the_device_counts_with_its_value_of_the_call(ops):
     scale.fill_(0.5)
     b = ops.long_attention(q, q, q, scale=scale)
     assert torch.equal(a, ops.long_attention(q, q, q, scale=0.125)) and torch.equal(b, ops.long_attention(q, q, q, scale=0.5)) and not torch.equal(a, b)
+
+
+def _pass(ops, q, k, v, dout, table):
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, table)]
+    out = ops.long_attention(*leaves[:3], causal=True, rel_table=leaves[3], rel_max=200, rel_bidirectional=False)
+    return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+
+def _wide(seed, S):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g).to(t).cuda() for s, t in (((1, S, 4, 128), BF16), ((1, S, 2, 128), BF16), ((1, S, 2, 128), BF16), ((1, S, 4, 128), BF16), ((24, 4), F32))]
+
+
+def test_captured_heads_of_128(ops):
+    """More than 64 KiB of LDS a block, split along the keys: recorded, and replayed with eager calls in between."""
+    args = _wide(1, 1500)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _pass(ops, *args)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = _pass(ops, *args)
+    for r in range(3):
+        for a, b in zip(args, _wide(5 + r, 1500)):
+            a.copy_(b)
+        g.replay()
+        want = _pass(ops, *args)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(res, want)), r
+
+
+def test_two_streams_at_once(ops):
+    """Passes that overlap on two streams share nothing: the bits of each are those of a pass alone."""
+    jobs = [_wide(1, 1500), _wide(2, 1100)]
+    want = [_pass(ops, *j) for j in jobs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for j, st in zip(jobs, streams):
+            with torch.cuda.stream(st):
+                got.append(_pass(ops, *j))
+    torch.cuda.synchronize()
+    for i, res in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(res, want[i % 2])), i

@@ -332,9 +332,9 @@ __global__ __launch_bounds__(256) void lp_bwd_kernel(LpP p) {
 template <typename T, bool TOP> int lp_fwd_launch(const LpP& p, hipStream_t st) {
   constexpr int CE = 16 / (int)sizeof(T);
   // a wave per row while a row fits its registers; short rows element by element (their vectors would be mostly partial); long rows of a launch that
-  // fills the chip a block of 256 each, of a small one a block of 1024 (8 x 30522 float32, top 5: 12.6 us, with 256: 31). The alternatives' kernel at
+  // fills the chip a block of 256 each, of a small one a block of 1024 (8 x 30522 float32, top 5: 12.6 us, with 256: 17.7). The alternatives' kernel at
   // five waves a SIMD: what it waits for are its own barriers, and 15 registers in memory cost less than the fourth wave's place (2048 x 30522 bf16,
-  // top 8: 53 us, unrestricted 88)
+  // top 8: 88 -> 58 us; 53 - 58 since passes are held against the list's last)
   if (p.V <= 512) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, 1, 8, TOP, 1>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
   else if (p.V <= 2048) hipLaunchKernelGGL((lp_fwd_kernel<T, 64, CE, 32 / CE, TOP, 1>), dim3(cdiv(p.rows, 4)), dim3(256), 0, st, p);
   else if (p.rows >= LP_MANY || p.V <= 8192) hipLaunchKernelGGL((lp_fwd_kernel<T, 256, CE, 32 / CE, TOP, TOP ? 5 : 1>), dim3(p.rows), dim3(256), 0, st, p);
