@@ -131,6 +131,8 @@ def _mask(kind, B, Sk, seed):
         m[-1] = -10000.0                                  # a sample whose every key is masked the finite way: plain softmax
     elif kind == "left":
         m = torch.where(j >= Sk - lens[:, None], 0.0, torch.finfo(F32).min)
+    elif kind == "leftpad":
+        m = torch.where(j >= Sk - lens[:, None], 0.0, float("-inf"))
     elif kind == "holes":
         m = torch.where(torch.rand((B, Sk), generator=g) < 0.3, float("-inf"), 0.0) + 0.5 * torch.randn((B, Sk), generator=g)
     return m.float().cuda()
@@ -182,11 +184,21 @@ def test_masks(ops, dtype, causal, mask, shape):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("mask,shape", [("leftpad", (3, 300, 300, 2, 1, 64)), ("leftpad", (2, 130, 333, 2, 2, 128)), ("leftpad", (4, 1, 500, 4, 2, 64)), ("holes", (2, 65, 200, 2, 1, 40)),
+                                        ("pad", (2, 100, 150, 2, 2, 96)), ("neg", (2, 100, 150, 2, 2, 32)), ("left", (2, 65, 200, 2, 1, 72)), ("leftpad", (2, 900, 900, 2, 2, 64))])
+def test_masks_at_other_sizes(ops, dtype, causal, mask, shape):
+    """Keys left out in front (whole tiles of them, rows that see none), and masks where head sizes are padded or rows are no power of two."""
+    _case(ops, dtype, shape, causal, mask, seed=17)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("shape,causal,mask,rel", [
     ((2, 70, 70, 2, 2, 64), False, "none", (32, 128, True)), ((1, 300, 300, 3, 3, 64), False, "pad", (8, 20, True)), ((1, 300, 300, 2, 2, 64), True, "none", (13, 37, False)),
     ((2, 50, 420, 4, 2, 128), True, "left", (16, 64, False)), ((1, 420, 50, 2, 1, 64), False, "empty", (10, 33, True)), ((1, 1, 700, 4, 2, 64), True, "none", (32, 128, False)),
     ((1, 3, 3, 1, 1, 8), False, "none", (4, 2, True)), ((1, 640, 640, 2, 2, 64), True, "holes", (32, 100, True)), ((1, 260, 260, 1, 1, 128), False, "none", (128, 1024, True)),
-    ((1, 130, 130, 2, 2, 32), False, "none", (2, 5, False)),
+    ((1, 130, 130, 2, 2, 32), False, "none", (2, 5, False)), ((2, 900, 900, 2, 1, 64), True, "leftpad", (24, 256, False)), ((2, 330, 500, 2, 2, 72), False, "pad", (32, 128, True)),
+    ((1, 500, 300, 2, 2, 96), True, "holes", (32, 128, True)),
 ])
 def test_learned_distance_bias(ops, dtype, shape, causal, mask, rel):
     _case(ops, dtype, shape, causal, mask, rel, seed=23)
