@@ -3569,7 +3569,7 @@ def _la_view(t):
 
 class _LaPlan:
     """What a call of one signature (shapes, types, options) needs besides its tensors; holds nothing of theirs."""
-    __slots__ = ("head", "first", "n_prep", "n_fwd", "n_bwd", "out_shape", "n_stat")
+    __slots__ = ("head", "first", "n_prep", "n_fwd", "n_bwd", "out_shape", "n_stat", "n_low")
 
 
 _LA_PLANS = {}
@@ -3609,6 +3609,7 @@ def _la_plan(q, k, v, kmask, table, causal, scale, rel_max, bidirectional):
     p.head = (dt, B, Sq, Sk, nh, nkv, D, int(bool(causal)), scale, 0 if p.first is None else len(p.first), sides,
               0 if p.first is None else ctypes.addressof(p.first))
     p.out_shape, p.n_stat = (B, Sq, nh, D), 2 * B * nh * Sq
+    p.n_low = 0 if q.dtype is torch.float32 else B * Sq * nh * D // 2      # (D is a multiple of 8: whole 16 bytes)
     p.n_prep = p.n_fwd = p.n_bwd = 0
     if min(B, Sq, Sk) > 0:
         sizes = (ctypes.c_long * 3)()
@@ -3644,13 +3645,14 @@ class _LongAttention(torch.autograd.Function):
         table = None if table is None else table.contiguous()
         n_stat, n_prep, n_fwd = plan.n_stat, plan.n_prep, plan.n_fwd
         out = q.new_empty(plan.out_shape)
-        low = q.new_empty(plan.out_shape) if train and q.dtype is not torch.float32 else None
-        keep = torch.empty((n_stat + n_prep,), dtype=torch.float32, device=q.device)                    # stat, then prep
+        n_low = ctx.n_low = plan.n_low if train else 0
+        keep = torch.empty((n_low + n_stat + n_prep,), dtype=torch.float32, device=q.device)            # what rounding took from out, stat, prep
         work = torch.empty((n_fwd,), dtype=torch.float32, device=q.device) if n_fwd else None
-        stat = keep.data_ptr()
+        low = keep.data_ptr()
+        stat = low + 4 * n_low
         _call_on(dev, "vlni_long_attn_fwd", _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, *qs, *ks, *vs, 0, 0, 0, _p(kmask), _p(table),
-                                                          out.data_ptr(), _p(low), stat, stat + 4 * n_stat, n_prep, _p(work), n_fwd, 0, 0, 0, 0))
-        ctx.save_for_backward(q, k, v, kmask, table, out, low, keep)
+                                                          out.data_ptr(), low if n_low else 0, stat, stat + 4 * n_stat, n_prep, _p(work), n_fwd, 0, 0, 0, 0))
+        ctx.save_for_backward(q, k, v, kmask, table, out, keep)
         return out
 
     @staticmethod
@@ -3662,15 +3664,16 @@ class _LongAttention(torch.autograd.Function):
             q, k, v, table = ctx.saved_tensors
             return (*[torch.zeros(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((q, k, v, None, table), ng)], None, None)
         # (checkpointing and offloading hand back other tensors than were saved, in other layouts: no address or stride of the forward pass holds)
-        q, k, v, kmask, table, out, low, keep = ctx.saved_tensors
+        q, k, v, kmask, table, out, keep = ctx.saved_tensors
         (q, qs), (k, ks), (v, vs), (dout, ds) = _la_view(q), _la_view(k), _la_view(v), _la_view(dout)
         kmask, table = None if kmask is None else kmask.contiguous(), None if table is None else table.contiguous()
-        out, low, stat = out.contiguous(), None if low is None else low.contiguous(), keep.data_ptr()
+        out, n_low, low = out.contiguous(), ctx.n_low, keep.data_ptr()
+        stat = low + 4 * n_low
         dq, dk, dv = q.new_empty(plan.out_shape), q.new_empty(k.shape), q.new_empty(k.shape)
         dtable = torch.empty_like(table) if ng[4] else None
         work = torch.empty((plan.n_bwd,), dtype=torch.float32, device=q.device)
         args = _LA_ARGS.pack(*plan.head, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *qs, *ks, *vs, *ds, _p(kmask), _p(table),
-                             out.data_ptr(), _p(low), stat, stat + 4 * plan.n_stat, plan.n_prep, work.data_ptr(), plan.n_bwd,
+                             out.data_ptr(), low if n_low else 0, stat, stat + 4 * plan.n_stat, plan.n_prep, work.data_ptr(), plan.n_bwd,
                              dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(dtable))
         _call_on(q.get_device(), "vlni_long_attn_bwd", args)
         return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, None, dtable, None, None
