@@ -128,7 +128,7 @@ int la_kt_of(const VlniLongAttnArgs* a) { return a->dtype == VLNI_F32 && a->D > 
 // products leave other blocks nothing to fill
 void la_tile(const VlniLongAttnArgs* a, bool keys, double (&tile)[2]) {
   const int dp = (a->D + 31) / 32 * 32;
-  if (a->dtype == VLNI_F32) tile[0] = tile[1] = (keys ? 12.5 : 6.0) * dp / 64 * la_kt_of(a) / 64;
+  if (a->dtype == VLNI_F32) tile[0] = tile[1] = (keys ? 10.5 : 6.0) * dp / 64 * la_kt_of(a) / 64;
   else {
     tile[0] = (keys ? 1.2 : 0.72) * (64 + dp) / 128;
     tile[1] = (keys ? 2.4 : 1.7) * (64 + dp) / 128;
