@@ -1,4 +1,4 @@
-// Shared by long_attention.hip (entry points, bfloat16, float16) and long_attention_f32.hip.
+// Shared by the long_attention*.hip files: one instance of the kernels per type, the entry points in long_attention.hip.
 #pragma once
 #include "common.h"
 
