@@ -109,7 +109,7 @@ int la_fill(const VlniLongAttnArgs* a, LaP& p, LaBuckets& k) {
 // Without a causal border all blocks are alike and run in rounds of one block a CU - two where a few rows leave the loads of K and V as the bound
 // (latency: a second block's loads fly under the first one's). With one, the chip works through half of the tiles on average (`part`) but waits for the
 // end of the longest chain. Splits cost a launch and their partial results, float32, written and read again at 4.5 TB/s.
-// Measured (heads of 64, whole -> split, with what joins them): dK / dV of a causal 4 k pass with four key heads, 256 blocks: 406 us -> in four 141 + 13;
+// Measured (heads of 64, whole -> split, with what joins them): dK / dV of a causal 4 k pass with four key heads, 256 blocks: 406 us -> in four 129 + 11;
 // 3 x 1501 causal positions of 8 heads with a bias, 288 blocks, forward: 42 -> in three 27 + 9; 1024 positions of 12 heads, 96 blocks, forward: 25 -> in
 // four 15 + 5; 2 x 512: 14 -> in two 12 + 5, so not split. A token over 8 k keys, 64 blocks of heads of 128: in eight 45 + 5, in 25 71.
 int la_split(double blocks, double chain, double part, bool few, const double (&tile)[2], double floats) {
