@@ -208,7 +208,6 @@ __global__ __launch_bounds__(TPB < 256 ? 256 : TPB, WPE) void lp_fwd_kernel(LpP 
         }
         lp_sync<NW>();
       } else {
-        if (tid == 0) q.count = 0;
         unsigned taken = 0;                                        // of this thread's vectors; the single element: out
         bool out = ie < 0;
         auto best = [&]() {                                        // largest value first, then its lowest index: no 64-bit key per element
@@ -250,6 +249,7 @@ __global__ __launch_bounds__(TPB < 256 ? 256 : TPB, WPE) void lp_fwd_kernel(LpP 
             wmax = lp_wave_max(mine);
           }
         }
+        if (tid == 0) q.count = 0;             // (behind the loop's barriers: every wave has read it and taken this branch)
         lp_sync<NW>();
       }
     }
