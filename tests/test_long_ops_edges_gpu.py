@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from tests.test_long_attention_gpu import _check, _reference, _run
+
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 INF = float("inf")
@@ -48,3 +50,19 @@ def test_ties_in_every_pass_of_long_rows(ops, dtype, rows, V):
     assert ((ent.double() - H).abs() <= err * (3 + H)).all()
     again = ops.token_logprobs(x, t, top=top)
     assert all(torch.equal(a, b) for a, b in zip(again, (logp, ent, tl, ti)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("S,lens,rel,causal", [(1024, (200, 1024, 70), (16, 40, True), False), (1500, (1, 640), (32, 91, True), False), (1024, (300, 900), (13, 37, False), False),
+                                               (900, (64, 500), (16, 40, False), True)])
+def test_table_gradient_of_rows_whose_near_keys_are_all_masked(ops, dtype, S, lens, rel, causal):
+    """Whole row blocks see valid keys beyond the last bucket's distance only: the band around them holds nothing but masked keys."""
+    B, nh, D = len(lens), 2, 64
+    q, k, v, dout = (_rand((B, S, nh, D), dtype, 31 + x) for x in range(4))
+    km = torch.where(torch.arange(S)[None] < torch.tensor(lens)[:, None], 0.0, -INF).float().cuda()
+    nb, rel_max, bidir = rel
+    table = _rand((nb, nh), F32, 40, 0.7)
+    got = _run(ops, q, k, v, dout, km, causal, table, rel_max, bidir)
+    _check(got, _reference(q, k, v, dout, km, causal, D ** -0.5, table, rel_max, bidir), (dtype, S, lens, rel))
+    again = _run(ops, q, k, v, dout, km, causal, table, rel_max, bidir)
+    assert all(torch.equal(got[n], again[n]) for n in got)
