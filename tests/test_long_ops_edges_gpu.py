@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_long_attention_gpu import _check, _reference, _run
+from tests.test_long_attention_gpu import _bucket, _check, _reference, _run
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -66,3 +66,131 @@ def test_table_gradient_of_rows_whose_near_keys_are_all_masked(ops, dtype, S, le
     _check(got, _reference(q, k, v, dout, km, causal, D ** -0.5, table, rel_max, bidir), (dtype, S, lens, rel))
     again = _run(ops, q, k, v, dout, km, causal, table, rel_max, bidir)
     assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+def _left(B, S, low):
+    """Keys in front of a sample's text carry `low`: S, S - S // 3, ... valid ones at the end."""
+    lens = torch.tensor([max(1, S - b * (S // 3)) for b in range(B)])
+    return torch.where(torch.arange(S)[None] >= S - lens[:, None], 0.0, low).float().cuda()
+
+
+def _by_row(q, k, v, dout, kmask, causal, scale, table=None, rel_max=0, bidir=True):
+    """float64 results with elementwise bounds as in test_long_attention_gpu, but with every row's own error of P: from the scores and the maximum among the keys
+    that have a share in it. Masks of -1e8 and less absorb scores below 32 in float32 (half a step of 1.4e8 is 8 in units of log2 already at 2^28): such a key's t is the mask itself, and
+    a row of nothing else has no rounding in its t at all."""
+    dt = q.dtype
+    u = torch.finfo(dt).eps / 2
+    up, tiny, e24 = (0.0 if dt == F32 else u), (2.0 ** -25 if dt == F16 else 0.0), 2.0 ** -24
+    B, Sq, nh, D = q.shape
+    Sk, nkv = k.shape[1], k.shape[2]
+    G = nh // nkv
+    f = lambda t: t.detach().double().transpose(1, 2)
+    Q, K, V, dO = f(q), f(k).repeat_interleave(G, 1), f(v).repeat_interleave(G, 1), f(dout)
+    i, j = torch.arange(Sq, device=q.device)[:, None], torch.arange(Sk, device=q.device)[None]
+    add = torch.zeros((B, 1, 1, Sk), dtype=torch.float64, device=q.device) if kmask is None else kmask.double()[:, None, None]
+    seen = (add > -INF).expand(B, 1, Sq, Sk)
+    if causal:
+        seen = seen & (j <= i + Sk - Sq)
+    t = scale * Q @ K.transpose(2, 3)
+    mag = scale * Q.abs() @ K.abs().transpose(2, 3)
+    if table is not None:
+        which = _bucket(j - (i + Sk - Sq), table.shape[0], rel_max, bidir)
+        t = t + table.detach().double().t()[:, which][None]
+    far = add <= -1e8
+    assert not far.any() or (t.abs().max() < 32 and add[far].max() <= -1e9)
+    t = torch.where(far, add.clamp(min=-1e30), t + add)
+    t = torch.where(seen, t, torch.full_like(t, -INF))
+    some = seen.any(-1, keepdim=True)
+    m = torch.where(some, t.amax(-1, keepdim=True), torch.zeros_like(t[..., :1]))
+    P = torch.where(seen, torch.exp(t - m), torch.zeros_like(t))
+    P = P / torch.where(some, P.sum(-1, keepdim=True), torch.ones_like(m))
+    share = (P > 2.0 ** -40) & ~far
+    zero = torch.zeros_like(t)
+    epsP = 2 * e24 * (D * torch.where(share, mag, zero).amax(-1, keepdim=True) + 8 * torch.where(share, t.abs(), zero).amax(-1, keepdim=True)) + 2.0 ** -20
+    nk, nq = (Sk + 8) * e24, (Sq * G + 8) * e24
+    out, aV = P @ V, P @ V.abs()
+    eO = (up + epsP + nk) * aV + u * out.abs() + tiny * V.abs().sum(2, keepdim=True)
+    res = {"out": (out, eO)}
+    dP, delta = dO @ V.transpose(2, 3), (dO * out).sum(-1, keepdim=True)
+    eD = eO if dt == F32 else eO - (u - u * u) * out.abs()
+    edelta = (dO.abs() * (eD + D * e24 * out.abs())).sum(-1, keepdim=True)
+    dS = P * (dP - delta)
+    aS, prod = dS.abs(), D * e24 * (dO.abs() @ V.abs().transpose(2, 3)) + 4 * e24 * (dP.abs() + delta.abs())
+    eS = up * aS + epsP * aS + P * (edelta + prod) + tiny * seen
+    dQ = scale * dS @ K
+    res["dq"] = (dQ, scale * ((eS + nk * aS) @ K.abs()) + u * dQ.abs())
+    dK, eK = scale * dS.transpose(2, 3) @ Q, scale * ((eS + nq * aS).transpose(2, 3) @ Q.abs())
+    dV, eV = P.transpose(2, 3) @ dO, ((up + epsP + nq) * P + tiny * seen).transpose(2, 3) @ dO.abs()
+    for n, g, e in (("dk", dK, eK), ("dv", dV, eV)):
+        g, e = g.view(B, nkv, G, Sk, D).sum(2), e.view(B, nkv, G, Sk, D).sum(2)
+        res[n] = (g, e + u * g.abs())
+    res = {n: (a.transpose(1, 2), b.transpose(1, 2) + tiny + 1e-30) for n, (a, b) in res.items()}
+    if table is not None:
+        row = ((epsP + nk) * (aS + P * edelta)).sum(-1, keepdim=True)
+        eS = epsP * aS + P * (row + prod) + (B * Sq + Sk) * e24 * aS
+        gt, et = torch.zeros_like(table, dtype=torch.float64), torch.zeros_like(table, dtype=torch.float64)
+        for b in range(table.shape[0]):
+            w = (which == b)
+            gt[b], et[b] = (dS * w).sum((0, 2, 3)), (eS * w).sum((0, 2, 3))
+        res["dtable"] = (gt, et + e24 * gt.abs() + 1e-30)
+    return res
+
+
+LOWS = [-1e4, -65504.0, -1e6, -1e9, -1e12, -1e19, -1e25, torch.finfo(F32).min]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("low", LOWS)
+@pytest.mark.parametrize("shape,causal,all_,rel", [((2, 300, 300, 4, 2, 64), True, False, None), ((2, 130, 750, 2, 2, 128), False, True, None), ((3, 200, 200, 2, 1, 64), True, False, (16, 40, False)),
+                                                   ((1, 1400, 1400, 1, 1, 32), True, True, None), ((2, 3, 900, 4, 1, 64), False, True, None)])
+def test_finite_masks_of_any_size(ops, dtype, low, shape, causal, all_, rel):
+    """Rows that see nothing but keys with a finite mask (every key of a sample, padding in front of a causal batch) are an ordinary softmax: the shares of a row add up to 1 in
+    the backward pass too - with an output gradient of ones, dV summed over the keys counts the rows. Where the mask absorbs the scores, and for -1e4, each value is held as well.
+    The sum's bound: P and its normalisation 2^-18 (m + log2(l) is kept in one float32 up to 64), n + rows additions of 2^-24, in 16 bits one rounding of P and one of dV."""
+    B, Sq, Sk, nh, nkv, D = shape
+    q, k, v, dout = (_rand(s, dtype, 3 + x) for x, s in enumerate([(B, Sq, nh, D), (B, Sk, nkv, D), (B, Sk, nkv, D), (B, Sq, nh, D)]))
+    km = torch.full((B, Sk), low, device="cuda") if all_ else _left(B, Sk, low)
+    nb, rel_max, bidir = rel or (0, 0, True)
+    table = _rand((nb, nh), F32, 9, 0.7) if rel else None
+    got = _run(ops, q, k, v, torch.ones_like(dout), km, causal, table, rel_max, bidir)
+    rows = Sq * (nh // nkv)
+    u = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+    bound = rows * (2.0 ** -18 + (Sk + rows) * 2.0 ** -24 + 2 * u) + (2.0 ** -25 * Sk * (rows + 1) if dtype == F16 else 0)
+    assert ((got["dv"].double().sum(1) - rows).abs() <= bound).all(), ((got["dv"].double().sum(1) - rows).abs().max().item(), bound)
+    if low in (-65504.0, -1e6):
+        return
+    got = _run(ops, q, k, v, dout, km, causal, table, rel_max, bidir)
+    _check(got, _by_row(q, k, v, dout, km, causal, D ** -0.5, table, rel_max, bidir), (dtype, low, shape, causal))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape,rel", [((3, 70, 70, 2, 1, 64), None), ((2, 130, 333, 2, 2, 128), None), ((3, 2, 400, 4, 1, 64), None), ((2, 300, 300, 2, 2, 64), (16, 40, True)), ((1, 900, 900, 1, 1, 40), None)])
+def test_rows_beside_masked_keys_to_their_own_bounds(ops, dtype, causal, shape, rel):
+    """-10000 on a sample's last keys: its rows' own scores are of order one, and so is their error."""
+    B, Sq, Sk, nh, nkv, D = shape
+    q, k, v, dout = (_rand(s, dtype, 13 + x) for x, s in enumerate([(B, Sq, nh, D), (B, Sk, nkv, D), (B, Sk, nkv, D), (B, Sq, nh, D)]))
+    lens = torch.tensor([Sk - b * (Sk // 4) - 1 for b in range(B)])
+    km = torch.where(torch.arange(Sk)[None] < lens[:, None], 0.0, -10000.0).float().cuda()
+    nb, rel_max, bidir = rel or (0, 0, True)
+    table = _rand((nb, nh), F32, 9, 0.7) if rel else None
+    _check(_run(ops, q, k, v, dout, km, causal, table, rel_max, bidir), _by_row(q, k, v, dout, km, causal, D ** -0.5, table, rel_max, bidir), (dtype, causal, shape))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("factor", [8.0, 300.0])
+def test_shares_add_up_at_large_scores(ops, dtype, factor):
+    """Scores of hundreds to ten thousands without a mask: the row's maximum leaves no room for log2(l) beside it in a float32."""
+    S, nh, D = 261, 16, 64
+    q, k, v = (_rand((1, S, nh, D), dtype, 3 + x) for x in range(3))
+    k[:, 1::3] = k[:, 2::3] = k[:, ::3]                              # every best key three times: shares of a third, and log2(3) beside the maximum
+    row = 16 * torch.arange(nh) + 2                                  # one row of each head has an output gradient, of ones
+    dout = torch.zeros_like(q)
+    dout[0, row, torch.arange(nh)] = 1.0
+    u = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+    for causal in (False, True):
+        got = _run(ops, q, k, v, dout, None, causal, None, 0, True, scale=factor)
+        # (a tile at the causal border rounds its scores once more, before the maximum is off them: 2^-24 of a |score| below 64 factor, twice)
+        bound = 2.0 ** -18 + 2 * S * 2.0 ** -24 + 2 * u + causal * 2 * 2.0 ** -24 * 64 * factor
+        off = (got["dv"].double().sum(1) - 1).abs().max().item()
+        assert off <= bound, (causal, off, bound)

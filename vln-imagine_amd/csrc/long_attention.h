@@ -4,7 +4,7 @@
 
 constexpr float LA_LOG2E = 1.4426950408889634f;
 constexpr float LA_LOWEST = -1e30f;          // finite masks below this count as this
-constexpr float LA_ABSORB = -1e20f;          // a running maximum below this came from such a mask
+constexpr float LA_FOLD = 64.f;              // a row whose maximum (in units of log2) is larger than this keeps 1 / sum apart from it
 constexpr int LA_PAD = 96;                   // a 32 x 64 piece that touches distance R reaches at most 94 beyond it
 constexpr int LA_MAXB = 64;                  // buckets per side
 
@@ -12,7 +12,7 @@ struct LaP {
   const void *q, *k, *v, *dout;
   long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, d_b, d_s, d_h;      // strides in elements
   void *out, *low;             // [B, Sq, nh, D] each: the result, and what its rounding to 16 bits took (null: nobody wants it)
-  float* lse; float* rl;       // [B, nh, Sq] each: see the masks' comment above
+  float* lse; float* rl;       // [B, nh, Sq] each: see the masks' comment in long_attention_impl.inc
   float* delta;                // [B, nh, Sq]
   const float* kml;            // [B, SkP] mask in units of log2, -inf behind Sk; null without a mask
   const int* kind;             // [B, SkP / 64]: 0 no mask in these 64 keys, 1 finite values, 2 nothing but -inf, 3 some -inf
