@@ -77,7 +77,9 @@ def _left(B, S, low):
 def _by_row(q, k, v, dout, kmask, causal, scale, table=None, rel_max=0, bidir=True):
     """float64 results with elementwise bounds as in test_long_attention_gpu, but with every row's own error of P: from the scores and the maximum among the keys
     that have a share in it. Masks of -1e8 and less absorb scores below 32 in float32 (half a step of 1.4e8 is 8 in units of log2 already at 2^28): such a key's t is the mask itself, and
-    a row of nothing else has no rounding in its t at all."""
+    a row of nothing else has no rounding in its t at all.
+    float16's smallest step: 2^-25 of a P in the forward pass and of a result; in the backward pass P is rounded times 2^12 and dS, whose size is
+    at most 2 D max|dO| max|V| P, times 2^12 and the power of two that brings that bound between 2 and 4 (max|dO|: of the row for dQ, of the sample and key head for dK)."""
     dt = q.dtype
     u = torch.finfo(dt).eps / 2
     up, tiny, e24 = (0.0 if dt == F32 else u), (2.0 ** -25 if dt == F16 else 0.0), 2.0 ** -24
@@ -116,11 +118,13 @@ def _by_row(q, k, v, dout, kmask, causal, scale, table=None, rel_max=0, bidir=Tr
     edelta = (dO.abs() * (eD + D * e24 * out.abs())).sum(-1, keepdim=True)
     dS = P * (dP - delta)
     aS, prod = dS.abs(), D * e24 * (dO.abs() @ V.abs().transpose(2, 3)) + 4 * e24 * (dP.abs() + delta.abs())
-    eS = up * aS + epsP * aS + P * (edelta + prod) + tiny * seen
+    eS = up * aS + epsP * aS + P * (edelta + prod)
+    rowmax, allmax = dO.abs().amax(-1, keepdim=True), dO.abs().reshape(B, nkv, -1).amax(-1).repeat_interleave(G, 1)[:, :, None, None]
+    least = 2.0 ** -12 * tiny * D * V.abs().amax((2, 3), keepdim=True) * seen
     dQ = scale * dS @ K
-    res["dq"] = (dQ, scale * ((eS + nk * aS) @ K.abs()) + u * dQ.abs())
-    dK, eK = scale * dS.transpose(2, 3) @ Q, scale * ((eS + nq * aS).transpose(2, 3) @ Q.abs())
-    dV, eV = P.transpose(2, 3) @ dO, ((up + epsP + nq) * P + tiny * seen).transpose(2, 3) @ dO.abs()
+    res["dq"] = (dQ, scale * ((eS + nk * aS + least * rowmax) @ K.abs()) + u * dQ.abs())
+    dK, eK = scale * dS.transpose(2, 3) @ Q, scale * ((eS + nq * aS + least * allmax).transpose(2, 3) @ Q.abs())
+    dV, eV = P.transpose(2, 3) @ dO, ((up + epsP + nq) * P + 2.0 ** -12 * tiny * seen).transpose(2, 3) @ dO.abs()
     for n, g, e in (("dk", dK, eK), ("dv", dV, eV)):
         g, e = g.view(B, nkv, G, Sk, D).sum(2), e.view(B, nkv, G, Sk, D).sum(2)
         res[n] = (g, e + u * g.abs())
@@ -194,3 +198,60 @@ def test_shares_add_up_at_large_scores(ops, dtype, factor):
         bound = 2.0 ** -18 + 2 * S * 2.0 ** -24 + 2 * u + causal * 2 * 2.0 ** -24 * 64 * factor
         off = (got["dv"].double().sum(1) - 1).abs().max().item()
         assert off <= bound, (causal, off, bound)
+
+
+def _spread(t, low):
+    """Rows of a tensor [B, S, ...] times powers of two from 1 down to `low`."""
+    n = torch.arange(t.shape[1], device=t.device) % 4
+    return (t.float() * (low ** (n / 3.0)).log2().round().exp2().view(1, -1, 1, 1)).to(t.dtype)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape,rel", [((2, 1500, 1500, 2, 1, 64), None), ((1, 260, 3000, 2, 2, 128), None), ((3, 700, 700, 4, 2, 64), (16, 40, True)), ((2, 2, 2500, 4, 1, 64), None), ((2, 333, 333, 2, 2, 72), None)])
+@pytest.mark.parametrize("size", [1e-4, 1.0, "rows", "samples"])
+def test_float16_gradients_of_any_size(ops, causal, shape, rel, size):
+    """Output gradients far from one, all alike or with small rows or samples beside large ones: P and dS below float16's normal range as they stand."""
+    B, Sq, Sk, nh, nkv, D = shape
+    q, k, v, dout = (_rand(s, F16, 61 + x) for x, s in enumerate([(B, Sq, nh, D), (B, Sk, nkv, D), (B, Sk, nkv, D), (B, Sq, nh, D)]))
+    if size == "rows":
+        dout = _spread(dout, 2.0 ** -12)
+    elif size == "samples":
+        dout = (dout.float() * torch.tensor([2.0 ** -12, 1.0, 2.0 ** -6])[:B].view(-1, 1, 1, 1).cuda()).half()
+    else:
+        dout = (dout.float() * size).half()
+    km = _left(B, Sk, -INF) if not causal else None
+    nb, rel_max, bidir = rel or (0, 0, True)
+    table = _rand((nb, nh), F32, 9, 0.7) if rel else None
+    got = _run(ops, q, k, v, dout, km, causal, table, rel_max, bidir)
+    ref = _by_row(q, k, v, dout, km, causal, D ** -0.5, table, rel_max, bidir)
+    _check(got, ref, (shape, causal, size))
+
+
+def test_float16_gradients_beyond_its_range_inside(ops):
+    """dS of 1e5 under results that float16 holds: not representable as it stands."""
+    B, Sq, Sk, nh, D, scale = 1, 24, 90, 2, 64, 1 / 16
+    q, k, v, dout = (_rand((B, S, nh, D), F16, 71 + x, c) for x, (S, c) in enumerate([(Sq, 2.0), (Sk, 2.0), (Sk, 8.0), (Sq, 3000.0)]))
+    ref = _by_row(q, k, v, dout, None, False, scale)
+    assert all(val.abs().max() < 6e4 for val, _ in ref.values())
+    Q, K, V, dO = (t.double().transpose(1, 2) for t in (q, k, v, dout))
+    P, g = torch.softmax(scale * Q @ K.transpose(2, 3).contiguous(), -1), dO @ V.transpose(2, 3).contiguous()
+    assert (P * (g - (P * g).sum(-1, keepdim=True))).abs().max() > 7e4
+    _check(_run(ops, q, k, v, dout, None, False, None, 0, True, scale=scale), ref, "large")
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_float16_excluded_keys_do_not_set_the_scale(ops, causal):
+    """Keys left out hold infinities, NaN and the largest number; their values are no part of what the gradients are scaled by."""
+    B, S, nh, D = 2, 400, 2, 64
+    q, k, v, dout = (_rand((B, S, nh, D), F16, 81 + x) for x in range(4))
+    dout = (dout.float() * 1e-3).half()
+    km = torch.where(torch.rand((B, S), generator=torch.Generator().manual_seed(1)) < 0.3, -INF, 0.0)
+    km[:, 0] = 0.0
+    km = km.cuda()
+    want = _run(ops, q, k, v, dout, km, causal, None, 0, True)
+    gone = km == -INF
+    k2, v2 = k.clone(), v.clone()
+    k2[gone], v2[gone] = float("nan"), 65504.0
+    v2[:, :, 1][gone] = INF
+    got = _run(ops, q, k2, v2, dout, km, causal, None, 0, True)
+    assert all(torch.equal(got[n], want[n]) for n in want)

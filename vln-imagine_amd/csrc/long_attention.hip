@@ -98,6 +98,9 @@ int la_fill(const VlniLongAttnArgs* a, LaP& p, LaBuckets& k) {
     VLNI_CHECK(p.R <= 1024, VLNI_EUNSUP, "long_attn: the last bucket begins at distance %d (at most 1024)", p.R);
     p.BL = 2 * p.R + 1 + 2 * LA_PAD;
   }
+  // float16: pieces of la_range_kernel, at most one a lane and at least 1024 reads of 16 bytes each
+  const long reads = (a->Sk > (long)a->Sq * (a->nh / a->nkv) ? a->Sk : (long)a->Sq * (a->nh / a->nkv)) * (a->D / 8);
+  p.nch = a->dtype != VLNI_F16 ? 0 : reads >= 65536 ? 64 : reads <= 1024 ? 1 : (int)(reads / 1024);
   // a few rows that share keys are worked on side by side (row = position x head of the group): one pass over K and V instead of one per head.
   // A bias differs by head, so its launches keep the heads apart.
   p.PG = !a->rel_table && (long)a->Sq * (a->nh / a->nkv) <= 128 ? a->nh / a->nkv : 1;
@@ -160,7 +163,7 @@ void la_prep_pointers(const VlniLongAttnArgs* a, LaP& p) {
   }
   if (a->rel_table) p.bvec = f;
 }
-// floats of workspace: forward: split results; backward: delta, row sums, sums by distance, split results (of dQ, then of dK and dV)
+// floats of workspace: forward: split results; backward: delta, ranges (float16), row sums, sums by distance, split results (of dQ, then of dK and dV)
 long la_fwd_work(const VlniLongAttnArgs* a, LaP p) {
   la_grid_rows(a, p);
   const long n = (long)p.B * p.Sq * p.nh;
@@ -169,6 +172,8 @@ long la_fwd_work(const VlniLongAttnArgs* a, LaP p) {
 long la_bwd_work(const VlniLongAttnArgs* a, LaP p, long* o_rs, long* o_db, long* o_part) {
   const long n = (long)p.B * p.Sq * p.nh;
   long f = (n + 3) & ~3L;
+  f += 2L * p.nch * p.B * p.nkv;
+  f = (f + 3) & ~3L;
   la_grid_rows(a, p);
   *o_rs = f;
   if (a->rel_table) f += 5 * p.nsplit * n;
@@ -272,6 +277,7 @@ extern "C" int vlni_long_attn_bwd(const VlniLongAttnArgs* a, void* stream) {
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   float* f = (float*)a->work;
   p.delta = f;
+  p.range = f + ((n + 3) & ~3L);
   p.rowsum = a->dtable ? f + o_rs : nullptr;
   p.dbpart = f + o_db;
   p.part = f + o_part;
