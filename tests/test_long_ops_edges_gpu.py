@@ -255,3 +255,18 @@ def test_float16_excluded_keys_do_not_set_the_scale(ops, causal):
     v2[:, :, 1][gone] = INF
     got = _run(ops, q, k2, v2, dout, km, causal, None, 0, True)
     assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("V", [37, 1500, 5000])
+def test_large_entropy_gradients_beside_impossible_entries(ops, V):
+    """A loss scale of 2^40 on the entropy term: entries of -inf have no gradient, whatever the factor."""
+    x = _rand((4, V), F32, 5)
+    x[:, ::3] = -INF
+    t = torch.ones(4, dtype=torch.int64, device="cuda")
+    def grad(c):
+        lg = x.clone().requires_grad_(True)
+        logp, ent, _, _ = ops.token_logprobs(lg, t)
+        return torch.autograd.grad([logp, ent], [lg], [torch.full((4,), c, device="cuda"), torch.full((4,), -c, device="cuda")])[0]
+    one, big = grad(1.0), grad(2.0 ** 40)
+    assert torch.isfinite(big).all() and (big[:, ::3] == 0).all()
+    assert torch.equal(big, one * 2.0 ** 40)                         # powers of two are exact

@@ -309,7 +309,7 @@ __global__ __launch_bounds__(256) void lp_bwd_kernel(LpP p) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       const float lp = (x[j] - m) - logl, pr = __builtin_amdgcn_exp2f(lp * LP_LOG2E);
-      float d = -pr * (g + h * (fmaxf(lp, -1e30f) + H));
+      float d = -pr * (g + h * (fmaxf(lp, -200.f) + H));              // (below -104 p is 0: no infinity may stand beside it, however large h)
       if (e + j == t) d += g;
       v[j] = (T)(dead ? 0.f : d);
     }
