@@ -270,3 +270,21 @@ def test_large_entropy_gradients_beside_impossible_entries(ops, V):
     one, big = grad(1.0), grad(2.0 ** 40)
     assert torch.isfinite(big).all() and (big[:, ::3] == 0).all()
     assert torch.equal(big, one * 2.0 ** 40)                         # powers of two are exact
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_masks_up_to_the_types_largest_value(ops, dtype):
+    """A key with the largest mask of all takes the whole row; -inf beside it leaves its key out."""
+    B, S, nh, D = 2, 130, 2, 64
+    q, k, v, dout = (_rand((B, S, nh, D), dtype, 21 + x) for x in range(4))
+    km = torch.zeros((B, S), device="cuda")
+    km[:, 77], km[:, 3] = torch.finfo(F32).max, -INF
+    got = _run(ops, q, k, v, dout, km, False, None, 0, True)
+    assert torch.equal(got["out"], v[:, 77:78].expand_as(v))
+    assert (got["dv"][:, :77] == 0).all() and (got["dv"][:, 78:] == 0).all()
+    # one share of 1: dS = <dO, v> - <dO, out> with out = v, which differ by the roundings of two sums of D products, D 2^-24 of their magnitudes each
+    # (out is exact), and the results by one rounding more
+    off = 2 * D * 2.0 ** -24 * (dout.double().abs() * v.double()[:, 77:78].abs()).sum(-1, keepdim=True) * D ** -0.5 * (1 + 2 * torch.finfo(dtype).eps)
+    assert (got["dq"].double().abs() <= off * k.double()[:, 77:78].abs()).all()
+    rest = torch.arange(S, device="cuda") != 77
+    assert (got["dk"][:, rest] == 0).all() and (got["dk"].double().abs()[:, 77] <= (off * q.double().abs()).sum(1)).all()

@@ -32,7 +32,7 @@ __global__ __launch_bounds__(64) void la_prep_kernel(const float* kmask, const f
     float v = -INFINITY;
     if (j < Sk) {
       v = kmask[(long)b * Sk + j];
-      if (v != -INFINITY) v = (v < LA_LOWEST ? LA_LOWEST : v) * LA_LOG2E;      // (NaN and +inf stay)
+      if (fabsf(v) != INFINITY) v = (v < -LA_MOST ? -LA_MOST : v > LA_MOST ? LA_MOST : v) * LA_LOG2E;      // (NaN stays)
     }
     kml[(long)b * SkP + j] = v;
     const bool none = __all(v == 0.f), all = __all(v == -INFINITY), some = __any(v == -INFINITY);
