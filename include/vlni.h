@@ -407,7 +407,7 @@ int vlni_ffn_block_bwd(const VlniBlockArgs* a, void* stream);
  * q [B,Sq,nh,D], k / v [B,Sk,nkv,D] with strides (elements) of sample, position and head, the D values of a head contiguous; nh a multiple of nkv
  * (query head h reads key head h nkv / nh); D a multiple of 8 up to 128; pointers 16-byte aligned, strides multiples of 16 bytes (0 allowed).
  * out, dq [B,Sq,nh,D] and dk, dv [B,Sk,nkv,D] are dense. kmask [B,Sk] float32 or NULL: a key of -inf takes no part (its k and v are not looked at, its
- * gradients are 0), other values are added (finite ones beyond +-1e30 count as +-1e30). causal: keys j > i + Sk - Sq take no part. A row without keys: out 0.
+ * gradients are 0), other values are added (finite ones beyond +-1e30 count as +-1e30). causal: keys j > i + Sk - Sq take no part. A row without keys: out 0, no gradient, its q and dout are not looked at.
  * rel_table [rel_sides rel_n, nh] float32 or NULL: a learned bias by distance, never materialised. rel_first (HOST array, rel_n <= 64 entries): the smallest
  * distance of each of a side's buckets, rel_first[0] = 0, last entry <= 1024; rows [0, rel_n) for keys at or before the query, [rel_n, 2 rel_n) behind it
  * (rel_sides 2) - with rel_sides 1 keys behind the query count as distance 0.

@@ -288,3 +288,26 @@ def test_masks_up_to_the_types_largest_value(ops, dtype):
     assert (got["dq"].double().abs() <= off * k.double()[:, 77:78].abs()).all()
     rest = torch.arange(S, device="cuda") != 77
     assert (got["dk"][:, rest] == 0).all() and (got["dk"].double().abs()[:, 77] <= (off * q.double().abs()).sum(1)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("S,D,rel", [(300, 64, None), (200, 128, (16, 40, False)), (70, 40, None)])
+def test_rows_without_keys_may_hold_anything(ops, dtype, S, D, rel):
+    """Causal batch with keys left out in front: rows that see none come out as zeros, and send no gradient back, with NaN in their q and infinities in
+    their output's gradient."""
+    B, nh = 2, 2
+    q, k, v, dout = (_rand((B, S, nh, D), dtype, 91 + x) for x in range(4))
+    km = _left(B, S, -INF)
+    km[0, :S // 2 + 3] = -INF
+    dead = (km == -INF).long().cumprod(1).bool()                     # rows before a sample's first key
+    assert dead.any() and not dead.all()
+    dout[dead] = 0
+    nb, rel_max, bidir = rel or (0, 0, True)
+    table = _rand((nb, nh), F32, 9, 0.7) if rel else None
+    want = _run(ops, q, k, v, dout, km, True, table, rel_max, bidir)
+    q2, dout2 = q.clone(), dout.clone()
+    q2[dead], dout2[dead] = float("nan"), INF
+    got = _run(ops, q2, k, v, dout2, km, True, table, rel_max, bidir)
+    assert (got["out"][dead] == 0).all() and (got["dq"][dead] == 0).all()
+    for n in want:
+        assert torch.equal(got[n], want[n]), n

@@ -3701,7 +3701,7 @@ def long_attention(q, k, v, kmask=None, causal=False, scale=None, rel_table=None
     q [B, Sq, nh, D], k and v [B, Sk, nkv, D] (float32, bfloat16 or float16; D a multiple of 8 up to 128; any strides - views of a packed projection
     are read in place where they lie on 16-byte steps). nh may be a multiple of nkv: query head h reads key head h * nkv // nh. Returns [B, Sq, nh, D].
     kmask: additive float32 [B, Sk] as `additive_mask` makes it. -inf excludes a key altogether (its k and v may hold anything), finite values are
-        added; those beyond +-1e30 count as +-1e30. A row without any key gives zeros and sends no gradient back.
+        added; those beyond +-1e30 count as +-1e30. A row without any key gives zeros and sends no gradient back, whatever its q and its output's gradient hold.
     causal: position i sees the keys j <= i + Sk - Sq (the sequences end together: one new token against a cache is Sq = 1).
     rel_table: float32 [buckets, nh], a learned bias by the distance j - (i + Sk - Sq), looked up in the kernels and trained through them. Of the n
         buckets of a side the first n // 2 hold one distance each, the others are spread over log(distance) up to rel_max (<= 1024), the last holds all
