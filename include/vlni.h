@@ -407,7 +407,8 @@ int vlni_ffn_block_bwd(const VlniBlockArgs* a, void* stream);
  * q [B,Sq,nh,D], k / v [B,Sk,nkv,D] with strides (elements) of sample, position and head, the D values of a head contiguous; nh a multiple of nkv
  * (query head h reads key head h nkv / nh); D a multiple of 8 up to 128; pointers 16-byte aligned, strides multiples of 16 bytes (0 allowed).
  * out, dq [B,Sq,nh,D] and dk, dv [B,Sk,nkv,D] are dense. kmask [B,Sk] float32 or NULL: a key of -inf takes no part (its k and v are not looked at, its
- * gradients are 0), other values are added (finite ones beyond +-1e30 count as +-1e30). causal: keys j > i + Sk - Sq take no part. A row without keys: out 0, no gradient, its q and dout are not looked at.
+ * gradients are 0), other values are added (finite ones beyond +-1e30 count as +-1e30). causal: keys j > i + Sk - Sq take no part. A row without
+ * keys: out 0, no gradient, whatever its q and dout hold.
  * rel_table [rel_sides rel_n, nh] float32 or NULL: a learned bias by distance, never materialised. rel_first (HOST array, rel_n <= 64 entries): the smallest
  * distance of each of a side's buckets, rel_first[0] = 0, last entry <= 1024; rows [0, rel_n) for keys at or before the query, [rel_n, 2 rel_n) behind it
  * (rel_sides 2) - with rel_sides 1 keys behind the query count as distance 0.
@@ -415,7 +416,9 @@ int vlni_ffn_block_bwd(const VlniBlockArgs* a, void* stream);
  * their error adds about a tenth to that of the gradients. Float32 needs none.
  * stat [2,B,nh,Sq] float32, out, out_low and prep go from the forward to the backward call, with the same kmask / rel_* arguments. dtable [rel_sides rel_n, nh] float32 is
  * written (not added to) or NULL. vlni_long_attn_sizes: floats of prep, of the forward's and of the backward's work, for these shapes and pointers.
- * All sums run in a fixed order: equal calls give equal bits. Replaces the reference's materialised attention (R:100-134, R:326-353) for long inputs. */
+ * A launch holds at
+ * most 2^24 - 1 blocks (128 rows, or 128 keys, of a sample, head and split); more is refused. All sums run in a fixed order: equal calls give equal bits.
+ * Replaces the reference's materialised attention (R:100-134, R:326-353) for long inputs. */
 typedef struct VlniLongAttnArgs {
   int dtype, B, Sq, Sk, nh, nkv, D, causal;
   float scale;
@@ -436,7 +439,8 @@ int vlni_long_attn_bwd(const VlniLongAttnArgs* a, void* stream);
 /* Log probability of target[r] in row r of logits [rows, V] (row stride ld; any dtype, may hold -inf), the row's entropy, and the `top` (<= 16, <= V) largest
  * log probabilities with their indices (equal values: lowest index first): the scores a sampled rollout keeps per action (Categorical.log_prob / entropy,
  * r2r/agent_cmt.py:569-574). A target equal to ignore_index, or outside [0, V) (then counted, vlni_set_index_error_counter), has logp 0 and no gradient
- * through logp. A row of -inf only: logp -inf, entropy 0, no gradient. stat [rows, 3] goes to the backward call, which writes
+ * through logp. A row of -inf only: logp -inf, entropy 0, no gradient. V up to 2^28; fewer than 2^26 rows up to V = 2040, fewer than 2^24 beyond.
+ * stat [rows, 3] goes to the backward call, which writes
  *   dlogits = dlogp ([v = target] - p_v) - dentropy p_v (log p_v + H)        (dlogp / dentropy [rows] float32, either may be NULL). */
 int vlni_token_logprobs_fwd(int dtype, const void* logits, long ld, const long* target, long ignore_index, float* logp, float* entropy, float* stat,
                             float* top_logp, long* top_index, int top, int rows, int V, void* stream);

@@ -350,12 +350,15 @@ template <typename T> int lp_bwd_launch(const LpP& p, hipStream_t st) {
   VLNI_LAUNCH_CHECK();
   return VLNI_OK;
 }
+// a launch has less than 2^32 threads: 256 a row, 64 where four rows share a block (in both directions)
+bool lp_fits(int rows, int V) { return rows < (V <= 2040 ? 1 << 26 : 1 << 24); }
 }  // namespace
 
 extern "C" int vlni_token_logprobs_fwd(int dtype, const void* logits, long ld, const long* target, long ignore_index, float* logp, float* entropy,
                                        float* stat, float* top_logp, long* top_index, int top, int rows, int V, void* stream) {
   VLNI_CHECK(dtype >= VLNI_F32 && dtype <= VLNI_F16, VLNI_EINVAL, "token_logprobs: dtype %d", dtype);
   VLNI_CHECK(rows > 0 && V > 0 && V <= (1 << 28) && ld >= V, VLNI_EINVAL, "token_logprobs: rows=%d V=%d ld=%ld", rows, V, ld);
+  VLNI_CHECK(lp_fits(rows, V), VLNI_EUNSUP, "token_logprobs: %d rows of %d (at most 2^26 - 1 up to 2040 columns, 2^24 - 1 beyond)", rows, V);
   VLNI_CHECK(top >= 0 && top <= LP_MAXTOP && top <= V, VLNI_EUNSUP, "token_logprobs: top=%d of %d (at most %d)", top, V, LP_MAXTOP);
   VLNI_CHECK(logits && target && logp && entropy && stat && (!top || (top_logp && top_index)), VLNI_EINVAL, "token_logprobs: null pointer");
   LpP p{};
@@ -371,6 +374,7 @@ extern "C" int vlni_token_logprobs_bwd(int dtype, const float* dlogp, const floa
                                        long ignore_index, const float* stat, void* dlogits, long lddl, int rows, int V, void* stream) {
   VLNI_CHECK(dtype >= VLNI_F32 && dtype <= VLNI_F16, VLNI_EINVAL, "token_logprobs: dtype %d", dtype);
   VLNI_CHECK(rows > 0 && V > 0 && V <= (1 << 28) && ld >= V && lddl >= V, VLNI_EINVAL, "token_logprobs: rows=%d V=%d ld=%ld lddl=%ld", rows, V, ld, lddl);
+  VLNI_CHECK(lp_fits(rows, V), VLNI_EUNSUP, "token_logprobs: %d rows of %d (at most 2^26 - 1 up to 2040 columns, 2^24 - 1 beyond)", rows, V);
   VLNI_CHECK(logits && target && stat && dlogits, VLNI_EINVAL, "token_logprobs: null pointer");
   LpP p{};
   p.x = logits; p.ld = ld; p.target = target; p.ignore = ignore_index; p.stat = (float*)stat; p.rows = rows; p.V = V; p.g = dlogp; p.h = dentropy;

@@ -196,9 +196,19 @@ int la_operand(const char* what, const void* ptr, const long* s, int dtype) {
              s[1], s[2], what);
   return VLNI_OK;
 }
+// a launch has less than 2^32 threads: 2^24 blocks of 256 rows' or keys' work, of the joins, and of 64 for the mask
+int la_limits(const VlniLongAttnArgs* a, LaP p) {
+  la_grid_rows(a, p);
+  const long rows = (long)p.nblk * p.nsplit * p.B * (p.nh / p.PG), row4 = p.nsplit > 1 ? (long)p.B * p.Sq * p.nh * p.D / 4 : 0;
+  la_grid_keys(a, p);
+  const long keys = (long)p.nblk * p.nsplit * p.B * p.nkv, key4 = p.nsplit > 1 ? (long)p.B * p.Sk * p.nkv * p.D / 2 : 0;
+  const long prep = (a->kmask ? (long)p.B * (p.SkP >> 6) : 0) + (a->rel_table ? (long)p.nh * cdiv(p.BL, 64) : 0);
+  VLNI_CHECK(rows < (1L << 24) && keys < (1L << 24) && prep < (1L << 26) && row4 < 0xFFFFFF00L && key4 < 0xFFFFFF00L, VLNI_EUNSUP,
+             "long_attn: B=%d Sq=%d Sk=%d nh=%d nkv=%d is more than one launch holds (%ld and %ld blocks, at most 2^24 - 1)", p.B, p.Sq, p.Sk, p.nh, p.nkv,
+             rows, keys);
+  return VLNI_OK;
+}
 int la_go(const VlniLongAttnArgs* a, const LaP& p, int what, hipStream_t st) {
-  const long blocks = (long)p.nblk * p.nsplit * p.B * (what == 2 ? p.nkv : p.nh / p.PG);
-  VLNI_CHECK(blocks < (1L << 31), VLNI_EUNSUP, "long_attn: %ld blocks", blocks);
   return a->dtype == VLNI_F32 ? la_run_f32(p, what, st) : a->dtype == VLNI_BF16 ? la_run_bf16(p, what, st) : la_run_f16(p, what, st);
 }
 }  // namespace
@@ -208,6 +218,7 @@ int la_go(const VlniLongAttnArgs* a, const LaP& p, int what, hipStream_t st) {
 extern "C" int vlni_long_attn_sizes(const VlniLongAttnArgs* a, long* sizes) {
   LaP p; LaBuckets k;
   LA_TRY(la_fill(a, p, k));
+  LA_TRY(la_limits(a, p));
   long o1, o2, o3;
   sizes[0] = la_prep_floats(a, p);
   sizes[1] = la_fwd_work(a, p);
@@ -218,6 +229,7 @@ extern "C" int vlni_long_attn_sizes(const VlniLongAttnArgs* a, long* sizes) {
 extern "C" int vlni_long_attn_fwd(const VlniLongAttnArgs* a, void* stream) {
   LaP p; LaBuckets k;
   LA_TRY(la_fill(a, p, k));
+  LA_TRY(la_limits(a, p));
   LA_TRY(la_operand("q", a->q, a->q_stride, a->dtype));
   LA_TRY(la_operand("k", a->k, a->k_stride, a->dtype));
   LA_TRY(la_operand("v", a->v, a->v_stride, a->dtype));
@@ -232,7 +244,6 @@ extern "C" int vlni_long_attn_fwd(const VlniLongAttnArgs* a, void* stream) {
   la_prep_pointers(a, p);
   if (need) {
     const long blocks = (a->kmask ? (long)p.B * (p.SkP >> 6) : 0) + (a->rel_table ? (long)p.nh * cdiv(p.BL, 64) : 0);
-    VLNI_CHECK(blocks < (1L << 31), VLNI_EUNSUP, "long_attn: %ld blocks", blocks);
     hipLaunchKernelGGL(la_prep_kernel, dim3((unsigned)blocks), dim3(64), 0, st, a->kmask, a->rel_table, (float*)p.kml, (int*)p.kind, (float*)p.bvec, k, p.B,
                        p.Sk, p.SkP, p.nh, p.R, p.BL);
     VLNI_LAUNCH_CHECK();
@@ -251,6 +262,7 @@ extern "C" int vlni_long_attn_fwd(const VlniLongAttnArgs* a, void* stream) {
 extern "C" int vlni_long_attn_bwd(const VlniLongAttnArgs* a, void* stream) {
   LaP p; LaBuckets k;
   LA_TRY(la_fill(a, p, k));
+  LA_TRY(la_limits(a, p));
   LA_TRY(la_operand("q", a->q, a->q_stride, a->dtype));
   LA_TRY(la_operand("k", a->k, a->k_stride, a->dtype));
   LA_TRY(la_operand("v", a->v, a->v_stride, a->dtype));

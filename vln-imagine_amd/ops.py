@@ -3791,7 +3791,7 @@ def token_logprobs(logits, target, top=0, ignore_index=-100):
         raise ValueError(f"token_logprobs: target is {target.dtype} {tuple(target.shape)}, expected int64 {tuple(logits.shape[:-1])}")
     if not 0 <= top <= min(16, logits.shape[-1]):
         raise ValueError(f"token_logprobs: top = {top} of {logits.shape[-1]} (at most 16)")
-    if logits.shape[-1] > 1 << 28 or target.numel() >= 1 << 31:
-        raise ValueError(f"token_logprobs: logits {tuple(logits.shape)}: at most 2^28 columns and 2^31 - 1 rows")
+    if logits.shape[-1] > 1 << 28 or target.numel() >= (1 << 26 if logits.shape[-1] <= 2040 else 1 << 24):
+        raise ValueError(f"token_logprobs: logits {tuple(logits.shape)}: at most 2^28 columns, and 2^26 - 1 rows up to 2040 columns, 2^24 - 1 beyond")
     _same_device(logits, "logits", target=target)
     return _TokenLogprobs.apply(logits, target, int(top), int(ignore_index))
