@@ -34,7 +34,7 @@ int vlni_set_dropout_seed_base(const unsigned* device_ptr);
 /* Optional: a device-resident int that counts rows whose table index was out of range. The entry points that take caller-supplied row
    indices (vlni_embed_combine_fwd, vlni_scatter_add_rows, vlni_scatter_add_rows_small) never touch memory outside the table: such a row
    adds nothing, and - once a counter is registered - is counted, so the host can raise the way nn.Embedding (R:535-544, R:596-618) would,
-   when it chooses to look (no per-call device-to-host sync). NULL / never called = skipped silently. */
+   when it chooses to look (no per-call device-to-host sync). NULL / never called, or a launch on another device than the counter's = skipped silently. */
 int vlni_set_index_error_counter(int* device_ptr);
 /* Host -> device copy of a small launch table on `stream` (hipMemcpyAsync). From pinned host memory it may be recorded into a hipGraph
    capture (a memcpy node; the host bytes must stay alive and unchanged for the graph's life). */

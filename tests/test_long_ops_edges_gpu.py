@@ -311,3 +311,18 @@ def test_rows_without_keys_may_hold_anything(ops, dtype, S, D, rel):
     assert (got["out"][dead] == 0).all() and (got["dq"][dead] == 0).all()
     for n in want:
         assert torch.equal(got[n], want[n]), n
+
+
+def test_out_of_range_targets_are_counted_on_the_counters_device_only(ops):
+    """The counter lies on one device; the same call on another one must not write there, and one that follows on the first counts as before."""
+    ops.watch_index_errors()
+    ops.index_errors(raise_=False)
+    x, t = _rand((6, 50), F32, 1), torch.tensor([50, -1, 3, 49, -100, 1 << 40]).cuda()
+    want = ops.token_logprobs(x, t, top=3)
+    assert ops.index_errors(raise_=False) == 3
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device: nothing to be kept apart")
+    got = ops.token_logprobs(x.to("cuda:1"), t.to("cuda:1"), top=3)
+    assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(got, want)) and ops.index_errors(raise_=False) == 0
+    ops.token_logprobs(x, t)
+    assert ops.index_errors(raise_=False) == 3

@@ -30,9 +30,21 @@ extern "C" int vlni_set_dropout_seed_base(const unsigned* device_ptr) {
 // row indices (vlni_embed_combine_fwd, vlni_scatter_add_rows*) skip a row whose index is outside its table - no out-of-bounds access -
 // and count it here when a counter is registered, so the host can raise like nn.Embedding does (ops.index_errors()), at a time of
 // its choosing instead of a device-to-host sync per call.
+// A launch on another device than the counter's gets none: its kernels could not reach that memory.
 static int* g_index_errors = nullptr;
-int* vlni_index_error_counter() { return g_index_errors; }
+static int g_index_errors_dev = -1;           // -1: not known (no device here)
+int* vlni_index_error_counter() {
+  int dev = -1;
+  if (g_index_errors && g_index_errors_dev >= 0 && (hipGetDevice(&dev) != hipSuccess || dev != g_index_errors_dev)) return nullptr;
+  return g_index_errors;
+}
 extern "C" int vlni_set_index_error_counter(int* device_ptr) {
+  hipPointerAttribute_t at;
+  g_index_errors_dev = -1;
+  if (device_ptr) {
+    if (hipPointerGetAttributes(&at, device_ptr) == hipSuccess && at.type == hipMemoryTypeDevice) g_index_errors_dev = at.device;
+    else (void)hipGetLastError();
+  }
   g_index_errors = device_ptr;
   return VLNI_OK;
 }

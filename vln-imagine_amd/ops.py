@@ -3783,7 +3783,7 @@ def token_logprobs(logits, target, top=0, ignore_index=-100):
     float32 [...], float32 [...], float32 and int64 [..., top] (None with top = 0), the alternatives in falling order, equal ones by lowest index.
     logp and entropy are differentiable (policy gradient with entropy bonus, r2r/agent_cmt.py:569-574,702-744; masked-token losses), the alternatives
     are not. A target equal to ignore_index, or outside [0, V), has logp 0 and sends no gradient through it; the latter are counted
-    (`watch_index_errors` / `index_errors`). A row of -inf only: logp -inf, entropy 0, no gradient; one that holds NaN gives NaN. top <= 16."""
+    (`watch_index_errors` / `index_errors`) on the counter's device. A row of -inf only: logp -inf, entropy 0, no gradient; one that holds NaN gives NaN. top <= 16."""
     _dt(logits)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"token_logprobs: logits {tuple(logits.shape)}")
