@@ -326,3 +326,34 @@ def test_out_of_range_targets_are_counted_on_the_counters_device_only(ops):
     assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(got, want)) and ops.index_errors(raise_=False) == 0
     ops.token_logprobs(x, t)
     assert ops.index_errors(raise_=False) == 3
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("shape,rel", [((2, 700, 700, 4, 2, 64), (16, 40, False)), ((1, 3, 2000, 4, 1, 128), None)])
+def test_captured_with_statistics_apart(ops, dtype, shape, rel):
+    """Recorded forward and backward with padding of -1e9 in front (rows whose 1 / sum stays apart), float16's ranges among the launches; replayed on inputs of other sizes with
+    eager calls between."""
+    B, Sq, Sk, nh, nkv, D = shape
+    sizes = [(B, Sq, nh, D), (B, Sk, nkv, D), (B, Sk, nkv, D), (B, Sq, nh, D)]
+    q, k, v, dout = (_rand(s, dtype, 3 + x) for x, s in enumerate(sizes))
+    km = _left(B, Sk, -1e9)
+    nb, rel_max, bidir = rel or (0, 0, True)
+    table = _rand((nb, nh), F32, 9, 0.7) if rel else None
+    args = (q, k, v, dout, km, True, table, rel_max, bidir)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _run(ops, *args)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = _run(ops, *args)
+    for r, c in enumerate((1.0, 1e-3, 30.0)):
+        for t, s in zip((q, k, v, dout), sizes):
+            t.copy_(_rand(s, dtype, 50 + r))
+        dout.mul_(c)
+        km.copy_(_left(B, Sk, -INF if r == 2 else -1e6))
+        g.replay()
+        eager = _run(ops, *args)
+        torch.cuda.synchronize()
+        assert all(torch.equal(res[n], eager[n]) for n in eager), r
