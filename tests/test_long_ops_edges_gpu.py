@@ -291,12 +291,12 @@ def test_masks_up_to_the_types_largest_value(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("S,D,rel", [(300, 64, None), (200, 128, (16, 40, False)), (70, 40, None)])
-def test_rows_without_keys_may_hold_anything(ops, dtype, S, D, rel):
+@pytest.mark.parametrize("S,D,rel,nh,nkv", [(300, 64, None, 2, 2), (200, 128, (16, 40, False), 2, 2), (70, 40, None, 2, 2), (2500, 64, None, 2, 1), (9, 64, None, 8, 2), (1800, 96, (32, 300, False), 2, 1)])
+def test_rows_without_keys_may_hold_anything(ops, dtype, S, D, rel, nh, nkv):
     """Causal batch with keys left out in front: rows that see none come out as zeros, and send no gradient back, with NaN in their q and infinities in
     their output's gradient."""
-    B, nh = 2, 2
-    q, k, v, dout = (_rand((B, S, nh, D), dtype, 91 + x) for x in range(4))
+    B = 2
+    q, k, v, dout = (_rand((B, S, h, D), dtype, 91 + x) for x, h in enumerate((nh, nkv, nkv, nh)))
     km = _left(B, S, -INF)
     km[0, :S // 2 + 3] = -INF
     dead = (km == -INF).long().cumprod(1).bool()                     # rows before a sample's first key
