@@ -412,8 +412,8 @@ int vlni_ffn_block_bwd(const VlniBlockArgs* a, void* stream);
  * rel_table [rel_sides rel_n, nh] float32 or NULL: a learned bias by distance, never materialised. rel_first (HOST array, rel_n <= 64 entries): the smallest
  * distance of each of a side's buckets, rel_first[0] = 0, last entry <= 1024; rows [0, rel_n) for keys at or before the query, [rel_n, 2 rel_n) behind it
  * (rel_sides 2) - with rel_sides 1 keys behind the query count as distance 0.
- * out_low, like out, or NULL: what rounding to 16 bits took from out. With it the backward call's sums <dout, out> are exact to float32; without it
- * their error adds about a tenth to that of the gradients. Float32 needs none.
+ * out_low, like out, or NULL: what rounding to 16 bits took from out. With it the backward call's sums <dout, out> take out to
+ * twice its bits (bfloat16: 2^-18 of a value); without it their error adds about a tenth to that of the gradients. Float32 needs none.
  * stat [2,B,nh,Sq] float32, out, out_low and prep go from the forward to the backward call, with the same kmask / rel_* arguments. dtable [rel_sides rel_n, nh] float32 is
  * written (not added to) or NULL. vlni_long_attn_sizes: floats of prep, of the forward's and of the backward's work, for these shapes and pointers.
  * A launch holds at
