@@ -76,7 +76,7 @@ def _left(B, S, low):
 
 def _by_row(q, k, v, dout, kmask, causal, scale, table=None, rel_max=0, bidir=True):
     """float64 results with elementwise bounds as in test_long_attention_gpu, but with every row's own error of P: from the scores and the maximum among the keys
-    that have a share in it. Masks of -1e8 and less absorb scores below 32 in float32 (half a step of 1.4e8 is 8 in units of log2 already at 2^28): such a key's t is the mask itself, and
+    that have a share in it. Masks (and entries of the table) of -1e8 and less absorb scores below 32 in float32 (half a step of 1.4e8 is 8 in units of log2 already at 2^28): such a key's t is the mask itself, and
     a row of nothing else has no rounding in its t at all.
     float16's smallest step: 2^-25 of a P in the forward pass and of a result; in the backward pass P is rounded times 2^12 and dS, whose size is
     at most 2 D max|dO| max|V| P, times 2^12 and the power of two that brings that bound between 2 and 4 (max|dO|: of the row for dQ, of the sample and key head for dK)."""
@@ -90,6 +90,7 @@ def _by_row(q, k, v, dout, kmask, causal, scale, table=None, rel_max=0, bidir=Tr
     Q, K, V, dO = f(q), f(k).repeat_interleave(G, 1), f(v).repeat_interleave(G, 1), f(dout)
     i, j = torch.arange(Sq, device=q.device)[:, None], torch.arange(Sk, device=q.device)[None]
     add = torch.zeros((B, 1, 1, Sk), dtype=torch.float64, device=q.device) if kmask is None else kmask.double()[:, None, None]
+    bias = torch.zeros_like(add)
     seen = (add > -INF).expand(B, 1, Sq, Sk)
     if causal:
         seen = seen & (j <= i + Sk - Sq)
@@ -97,10 +98,10 @@ def _by_row(q, k, v, dout, kmask, causal, scale, table=None, rel_max=0, bidir=Tr
     mag = scale * Q.abs() @ K.abs().transpose(2, 3)
     if table is not None:
         which = _bucket(j - (i + Sk - Sq), table.shape[0], rel_max, bidir)
-        t = t + table.detach().double().t()[:, which][None]
-    far = add <= -1e8
-    assert not far.any() or (t.abs().max() < 32 and add[far].max() <= -1e9)
-    t = torch.where(far, add.clamp(min=-1e30), t + add)
+        bias = table.detach().double().t()[:, which][None]
+    far, far_m, far_b = (add <= -1e8) | (bias <= -1e8), add <= -1e8, bias <= -1e8
+    assert not far.any() or ((t + bias * ~far_b).abs().max() < 32 and (add * far_m + bias * far_b).where(far, -1e9).max() <= -1e9)
+    t = torch.where(far, torch.where(far_m, add.clamp(min=-1e30), 0.0) + torch.where(far_b, bias, 0.0), t + add + bias)
     t = torch.where(seen, t, torch.full_like(t, -INF))
     some = seen.any(-1, keepdim=True)
     m = torch.where(some, t.amax(-1, keepdim=True), torch.zeros_like(t[..., :1]))
@@ -357,3 +358,38 @@ def test_captured_with_statistics_apart(ops, dtype, shape, rel):
         eager = _run(ops, *args)
         torch.cuda.synchronize()
         assert all(torch.equal(res[n], eager[n]) for n in eager), r
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("S,lens,D,low", [(300, (300, 120), 64, -1e9), (700, (90, 700), 128, -1e9), (500, (200, 60), 40, -1e12)])
+def test_rows_that_see_only_distances_the_table_forbids(ops, dtype, S, lens, D, low):
+    """A window by the table (far buckets at -1e9) over a ragged batch: padded rows see nothing but far keys. Their scores are absorbed by the bias: every key has the same share."""
+    B, nh = len(lens), 2
+    q, k, v, dout = (_rand((B, S, nh, D), dtype, 41 + x) for x in range(4))
+    km = torch.where(torch.arange(S)[None] < torch.tensor(lens)[:, None], 0.0, -INF).float().cuda()
+    table = _rand((16, nh), F32, 9, 0.7)
+    table[7] = table[15] = low
+    got = _run(ops, q, k, v, dout, km, False, table, 30, True)
+    _check(got, _by_row(q, k, v, dout, km, False, D ** -0.5, table, 30, True), (dtype, S, lens))
+
+
+@pytest.mark.parametrize("dtype,size", [(F32, 3e3), (F32, 1e6), (BF16, 3e3), (BF16, 1e6), (F16, 3e3), (F16, 1e4)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_scores_far_beyond_a_float32s_steps(ops, dtype, size, causal):
+    """Scores of 1e7 to 1e14: the best key of a row takes it whole (rows whose two best lie closer than the scores' rounding, D 2^-24 of their magnitudes, are left out)."""
+    S, nh, D = 200, 2, 64
+    q, k, v, dout = (_rand((1, S, nh, D), dtype, 51 + x, c) for x, c in enumerate((size, size, 1.0, 1.0)))
+    t = q.double().transpose(1, 2) @ k.double().permute(0, 2, 3, 1) * D ** -0.5
+    if causal:
+        t = t.masked_fill(torch.arange(S, device="cuda")[None] > torch.arange(S, device="cuda")[:, None], -INF)
+    near = 4 * D * 2.0 ** -24 * (q.double().abs().transpose(1, 2) @ k.double().abs().permute(0, 2, 3, 1)).amax(-1) * D ** -0.5 + 60
+    two, best = t.topk(2, -1)
+    clear = two[..., 0] - two[..., 1] > near
+    assert clear.double().mean() > 0.9
+    got = _run(ops, q, k, v, dout, None, causal, None, 0, True)
+    want = v.transpose(1, 2).gather(2, best[..., :1].expand(-1, -1, -1, D))
+    assert torch.equal(got["out"].transpose(1, 2)[clear], want[clear])
+    assert all(torch.isfinite(g).all() for g in got.values())
+    # dS of such a row is <dO, v> - <dO, out>, the roundings of two equal sums, or 0
+    off = 2 * D * 2.0 ** -24 * (dout.double().abs().transpose(1, 2) * want.double().abs()).sum(-1) * D ** -0.5 * k.double().abs().max() * 1.01
+    assert (got["dq"].double().transpose(1, 2).abs()[clear] <= off[clear][:, None] + 2.0 ** -25).all()

@@ -6,6 +6,7 @@
 
 constexpr float LA_LOG2E = 1.4426950408889634f;
 constexpr float LA_MOST = 1e30f;             // finite masks beyond +- this count as this
+constexpr float LA_EXACT = 1048576.f;        // a row whose maximum is larger than this rounds its scores before the maximum is taken off them
 constexpr float LA_FOLD = 64.f;              // a row whose maximum (in units of log2) is larger than this keeps 1 / sum apart from it
 constexpr int LA_PAD = 96;                   // a 32 x 64 piece that touches distance R reaches at most 94 beyond it
 constexpr int LA_MAXB = 64;                  // buckets per side
